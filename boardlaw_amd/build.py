@@ -26,7 +26,10 @@ GEN_STAMP = GEN_LIB + '.torch'      # the torch version the shim was compiled ag
 
 # -ffp-contract=off: the search kernels must round like the reference's CPU path (no FMA); see DESIGN.md.
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-ffp-contract=off', '-fPIC', '-fno-gpu-flush-denormals-to-zero',
-         '-I' + os.path.join(ROOT, 'include')]
+         '-I' + os.path.join(ROOT, 'include'),
+         # no packed fp32 instructions (v_pk_add / mul / fma_f32, which -O3 makes of ordinary float code): some of their forms have
+         # given wrong results on these GPUs now and then.  The host pass of hipcc warns that it does not know the feature: harmless.
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # measurement builds only (tools/ab_build.sh: variants of a kernel's compile-time switches, e.g. BL_HIPCC_EXTRA=-DBLM_RD64=2)
 FLAGS += os.environ.get('BL_HIPCC_EXTRA', '').split()
 
