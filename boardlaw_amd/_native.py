@@ -13,7 +13,7 @@ LIBPATH = os.path.join(HERE, 'libboardlaw_amd.so')
 QRANGE_WORDS = 4096
 BL_OK, BL_EINVAL, BL_ETOOBIG, BL_ELAUNCH = 0, -1, -2, -3
 
-_vp, _i = ctypes.c_void_p, ctypes.c_int
+_vp, _i, _l = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
 
 
 class Tune(ctypes.Structure):
@@ -71,6 +71,14 @@ SYMBOLS = {
     'bl_copy_many': (_i, [_vp, _i, _vp]),
     'bl_rand_block': (_i, [_vp, _i, ctypes.c_long, ctypes.c_long, _i, ctypes.c_ulonglong, ctypes.c_ulonglong, ctypes.c_uint, _i, _i, _vp]),
     'bl_selftest': (_i, [_vp]),
+    'bl_logprobs_workspace': (_l, [_l, _i, _i]),
+    'bl_logprobs': (_i, [_vp, _i, _l, _vp, _l, _vp, _l, _i, _i] + [_vp] * 7),
+    'bl_logprobs_grad': (_i, [_vp, _i, _l, _vp, _l, _vp, _l, _i, _i] + [_vp] * 8),
+    'bl_norm_residual': (_i, [_vp, _i, _l, _vp, _i, _l, _vp, _vp, _vp, _i, _l, _vp, ctypes.c_float, _l, _i] + [_vp] * 4),
+    'bl_norm_residual_workspace': (_l, [_l, _i]),
+    'bl_norm_residual_grad': (_i, [_vp, _i, _l, _vp, _i, _l, _vp, _vp, _vp, _i, _l, _vp, ctypes.c_float, _l, _i] + [_vp, _vp, _l, _vp, _l, _vp, _vp, _l, _vp, _l] + [_vp] * 5),
+    'bl_orthogonalize_workspace': (_l, [_i, _i, _i]),
+    'bl_orthogonalize': (_i, [_vp, _vp, _i, _i, _i, _i, _i, ctypes.c_float, _vp, _vp]),
     'bl_powf2': (_i, [_vp, _vp, ctypes.c_long, _vp]),
 }
 
@@ -217,6 +225,21 @@ def copy_many(dsts, srcs):
 
 def ptr(t):
     return t.data_ptr()
+
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}        # BL_F32, BL_F16, BL_BF16
+TOP_MAX, NORM_MAX, ORTHO_MAX = 64, 8192, 16384
+
+
+def on(device):
+    """Context in which `device` is the current one."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def rows_of(t, width):
+    """`t` (..., width) as (rows, width) with a contiguous last dimension: a view where the layout allows one."""
+    t = t if t.ndim == 2 else t.reshape(-1, width)
+    return t if t.stride(1) == 1 or width == 1 else t.contiguous()
 
 
 def require_device(*tensors):

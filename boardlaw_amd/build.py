@@ -14,7 +14,8 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-UNITS = ('bl_search.hip', 'bl_sim.hip', 'bl_hex.hip', 'bl_abi.hip', 'bl_expand.hip', 'bl_rows.hip', 'bl_mlp.hip', 'bl_layers.hip', 'bl_root.hip', 'bl_rand.hip')
+UNITS = ('bl_search.hip', 'bl_sim.hip', 'bl_hex.hip', 'bl_abi.hip', 'bl_expand.hip', 'bl_rows.hip', 'bl_mlp.hip', 'bl_layers.hip', 'bl_root.hip', 'bl_rand.hip',
+         'bl_logprobs.hip', 'bl_norm.hip', 'bl_ortho.hip')
 SOURCES = [os.path.join(HERE, 'csrc', f) for f in UNITS]
 # every header under csrc/ (bl_device.h includes bl_powf.h, ...): editing any of them rebuilds every object
 HEADERS = [os.path.join(ROOT, 'include', 'boardlaw_amd.h')] + sorted(glob.glob(os.path.join(HERE, 'csrc', '*.h')))

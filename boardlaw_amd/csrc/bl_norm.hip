@@ -1,0 +1,367 @@
+// bl_norm.hip -- the residual stream between two blocks in one pass: norm behind the block, its gate, the residual scale, norm before
+// the next block; and the gradient.  Per row of W:
+//     n = y / rms(y),  u = sigmoid(gate) post n,  x' = x + alpha u,  h = pre x' / rms(x'),     rms(v) = sqrt(mean v^2 + eps)
+// Backward, with xn = x' / rms(x') recomputed from x and y (so it is not the rounded x' that is differentiated) and the two reciprocal
+// rms of the forward pass:
+//     z  = g_x' + rx (t - xn mean(t xn)),  t = g_h pre;      dx = z;      dpre = sum_rows g_h xn;      dalpha = sum z u
+//     dgate = alpha z post n s (1 - s);    dpost = sum_rows alpha z s n;  dy = ry (dn - n mean(dn n)),  dn = alpha z s post
+// Everything is computed in f32 and rounded once at its store.  The bound is HBM: every element is read once and written once; a row
+// is held in registers by G lanes of 8 elements each, so the two dependent sums of a row cost no second read.  The sums over rows are
+// kept per workgroup in registers over all of its rows and added up by a second launch in a fixed order: no atomics, the same bits
+// every time.
+#include "bl_train.h"
+
+#pragma clang fp contract(off)
+
+using namespace bltrain;
+
+namespace {
+
+constexpr int N = 8;                        // elements of a row per lane
+
+struct Norm {
+    const void* x; long xs;
+    const void* y; long ys;
+    const float* alpha; const float* post;
+    const void* gate; long gs; int kind;
+    const float* pre;
+    float eps, inv_w; long R; int W;
+    void* xo; void* h; float* stats;        // forward
+    const void* gx; long gxs; const void* gh; long ghs;          // backward
+    void* dx; void* dy; long dys; void* dgate; long dgs; float* parts;
+};
+
+// where lane gl's 8 elements of a row are: VEC == 8 together (16-byte accesses), VEC == 1 every G-th
+template <int G, int VEC> __device__ __forceinline__ int column(int gl, int i) { return VEC == 8 ? 8 * gl + i : gl + G * i; }
+
+template <int G, int VEC, typename T> __device__ __forceinline__ void read(const T* p, int gl, int W, float (&o)[N]) {
+    if constexpr (VEC == 8) {
+        if (8 * gl < W) load<T, 8>(p + 8 * gl, o);
+        else
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) { const int j = gl + G * i; o[i] = (float)p[j < W ? j : W - 1]; }
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = gl + G * i < W ? o[i] : 0.f;
+    }
+}
+template <int G, int VEC, typename T> __device__ __forceinline__ void write(T* p, int gl, int W, const float (&o)[N]) {
+    if constexpr (VEC == 8) {
+        if (8 * gl < W) store<T, 8>(p + 8 * gl, o);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) { const int j = gl + G * i; if (j < W) p[j] = (T)o[i]; }
+    }
+}
+
+// sum over the G lanes of a row, in every one of them.  G > 64: the row is a workgroup's; `lds` holds a value per wave, two sets of
+// them in turn (`set`), so that one barrier per sum is enough
+template <int G> __device__ __forceinline__ float row_sum(float v, float* lds, int& set) {
+    v = reduce<(G < 64 ? G : 64), Sum>(v);
+    if constexpr (G > 64) {
+        float* at = lds + 16 * set;
+        set ^= 1;
+        if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = at[0];
+#pragma unroll
+        for (int w = 1; w < G / 64; w++) v += at[w];
+    }
+    return v;
+}
+
+struct Gate { float s, ds; };               // sigmoid and its derivative
+__device__ __forceinline__ Gate sigmoid(float g) {
+    const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896341f), s = __builtin_amdgcn_rcpf(1.f + e);
+    return {s, s == 0.f ? 0.f : e * s * s};
+}
+
+template <typename TX, typename TY, int G, int VEC>
+__global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(Norm q) {
+    __shared__ float lds[32];
+    constexpr int T = G > 256 ? G : 256, ROWS = T / G;
+    const int gl = threadIdx.x & (G - 1);
+    int set = 0;
+    float post[N], pre[N], gate[N];
+    if (q.post) read<G, VEC>(q.post, gl, q.W, post);
+    if (q.pre) read<G, VEC>(q.pre, gl, q.W, pre);
+    if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
+    const float alpha = q.alpha ? *q.alpha : 1.f;
+    for (long r0 = (long)blockIdx.x * ROWS; r0 < q.R; r0 += (long)gridDim.x * ROWS) {
+        const long row = r0 + threadIdx.x / G, at = row < q.R ? row : q.R - 1;      // (G > 64: one row per workgroup, always live)
+        const bool live = row < q.R;
+        float x[N];
+        read<G, VEC>((const TX*)q.x + at * q.xs, gl, q.W, x);
+        float ry = 1.f;
+        if (q.y) {
+            float y[N];
+            read<G, VEC>((const TY*)q.y + at * q.ys, gl, q.W, y);
+            if (q.kind == BL_GATE_FULL) read<G, VEC>((const TY*)q.gate + at * q.gs, gl, q.W, gate);
+            if (q.kind == BL_GATE_ROW) {
+                const float g = (float)((const TY*)q.gate)[at * q.gs];
+#pragma unroll
+                for (int i = 0; i < N; i++) gate[i] = g;
+            }
+            if (q.post) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; i++) ss = fmaf(y[i], y[i], ss);
+                ry = __builtin_amdgcn_rsqf(row_sum<G>(ss, lds, set) * q.inv_w + q.eps);
+#pragma unroll
+                for (int i = 0; i < N; i++) y[i] *= post[i] * ry;
+            }
+            if (q.kind != BL_GATE_NONE)
+#pragma unroll
+                for (int i = 0; i < N; i++) y[i] *= sigmoid(gate[i]).s;
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] = fmaf(alpha, y[i], x[i]);
+            if (live) write<G, VEC>((TX*)q.xo + at * q.W, gl, q.W, x);
+        }
+        float rx = 1.f;
+        if (q.pre) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; i++) if (column<G, VEC>(gl, i) < q.W) ss = fmaf(x[i], x[i], ss);
+            rx = __builtin_amdgcn_rsqf(row_sum<G>(ss, lds, set) * q.inv_w + q.eps);
+            float h[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) h[i] = pre[i] * (x[i] * rx);
+            if (live) write<G, VEC>((TY*)q.h + at * q.W, gl, q.W, h);
+        }
+        if (q.stats && live && gl == 0) { q.stats[2 * at] = ry; q.stats[2 * at + 1] = rx; }
+    }
+}
+
+template <typename TX, typename TY, int G, int VEC>
+__global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
+    __shared__ float lds[32];
+    constexpr int T = G > 256 ? G : 256, ROWS = T / G;
+    __shared__ float cols[G <= 64 ? 3 * N * G + 1 : 1];
+    const int gl = threadIdx.x & (G - 1);
+    int set = 0;
+    float post[N], pre[N], gate[N];
+    if (q.post) read<G, VEC>(q.post, gl, q.W, post);
+    if (q.gh) read<G, VEC>(q.pre, gl, q.W, pre);
+    if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
+    const float alpha = q.alpha ? *q.alpha : 1.f;
+    float spost[N], spre[N], sgate[N], salpha = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++) spost[i] = spre[i] = sgate[i] = 0.f;
+    for (long r0 = (long)blockIdx.x * ROWS; r0 < q.R; r0 += (long)gridDim.x * ROWS) {
+        const long row = r0 + threadIdx.x / G, at = row < q.R ? row : q.R - 1;
+        const bool live = row < q.R;
+        const float ry = q.stats[2 * at], rx = q.stats[2 * at + 1];
+        float x[N], z[N], n[N], s[N], ds[N], u[N];
+        read<G, VEC>((const TX*)q.x + at * q.xs, gl, q.W, x);
+        if (q.y) {
+            read<G, VEC>((const TY*)q.y + at * q.ys, gl, q.W, n);
+            if (q.kind == BL_GATE_FULL) read<G, VEC>((const TY*)q.gate + at * q.gs, gl, q.W, gate);
+            if (q.kind == BL_GATE_ROW) {
+                const float g = (float)((const TY*)q.gate)[at * q.gs];
+#pragma unroll
+                for (int i = 0; i < N; i++) gate[i] = g;
+            }
+        }
+        float t[N];
+        if (q.gx) read<G, VEC>((const TX*)q.gx + at * q.gxs, gl, q.W, z);
+        else
+#pragma unroll
+            for (int i = 0; i < N; i++) z[i] = 0.f;
+        if (q.gh) read<G, VEC>((const TY*)q.gh + at * q.ghs, gl, q.W, t);
+        if (q.y) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                n[i] *= ry;
+                u[i] = q.post ? post[i] * n[i] : n[i];
+                if (q.kind != BL_GATE_NONE) { const Gate g = sigmoid(gate[i]); s[i] = g.s; ds[i] = g.ds; u[i] *= g.s; }
+                else { s[i] = 1.f; ds[i] = 0.f; }
+                x[i] = fmaf(alpha, u[i], x[i]);
+            }
+        }
+        if (q.gh) {
+            float c = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                x[i] *= rx;                                                          // xn
+                if (live) spre[i] = fmaf(t[i], x[i], spre[i]);
+                t[i] *= pre[i];
+                c = column<G, VEC>(gl, i) < q.W ? fmaf(t[i], x[i], c) : c;
+            }
+            c = row_sum<G>(c, lds, set) * q.inv_w;
+            // one column: xn^2 = 1 - eps rx^2, and the difference would cancel
+#pragma unroll
+            for (int i = 0; i < N; i++) z[i] = fmaf(rx, q.W == 1 ? t[i] * (q.eps * rx * rx) : fmaf(-x[i], c, t[i]), z[i]);
+        }
+        if (live) write<G, VEC>((TX*)q.dx + at * q.W, gl, q.W, z);
+        if (!q.y) continue;
+        float c = 0.f, cg = 0.f, dn[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const bool in = column<G, VEC>(gl, i) < q.W;
+            if (live && in) salpha = fmaf(z[i], u[i], salpha);
+            const float v = alpha * z[i], vn = v * n[i], p = q.post ? post[i] : 1.f;
+            dn[i] = v * s[i] * p;
+            if (live) spost[i] = fmaf(vn, s[i], spost[i]);
+            ds[i] *= vn * p;                                                         // dgate
+            if (live) sgate[i] += ds[i];
+            cg += in ? ds[i] : 0.f;
+            c = in ? fmaf(dn[i], n[i], c) : c;
+        }
+        if (q.post) {
+            c = row_sum<G>(c, lds, set) * q.inv_w;
+#pragma unroll
+            for (int i = 0; i < N; i++) dn[i] = ry * (q.W == 1 ? dn[i] * (q.eps * ry * ry) : fmaf(-n[i], c, dn[i]));
+        }
+        if (live) write<G, VEC>((TY*)q.dy + at * q.dys, gl, q.W, dn);
+        if (q.dgate && q.kind == BL_GATE_FULL && live) write<G, VEC>((TY*)q.dgate + at * q.dgs, gl, q.W, ds);
+        if (q.kind == BL_GATE_ROW) {
+            cg = row_sum<G>(cg, lds, set);
+            if (q.dgate && live && gl == 0) ((TY*)q.dgate)[at * q.dgs] = (TY)cg;
+        }
+    }
+    // this workgroup's sums over its rows: dpost, dpre, dgate per column, then dalpha
+    float* out = q.parts + (long)blockIdx.x * (3l * q.W + 1);
+    salpha = row_sum<G>(salpha, lds, set);
+    if constexpr (G > 64) {
+        if (T == G) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int j = column<G, VEC>(gl, i);
+                if (j < q.W) { out[j] = spost[i]; out[q.W + j] = spre[i]; out[2 * q.W + j] = sgate[i]; }
+            }
+            if (gl == 0) out[3 * q.W] = salpha;
+        }
+    } else {
+        // the workgroup's groups of lanes one after the other: a fixed order
+        for (int g = 0; g < ROWS; g++) {
+            if (threadIdx.x / G == g) {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const int k = gl + G * i;
+                    cols[k] = g ? cols[k] + spost[i] : spost[i];
+                    cols[N * G + k] = g ? cols[N * G + k] + spre[i] : spre[i];
+                    cols[2 * N * G + k] = g ? cols[2 * N * G + k] + sgate[i] : sgate[i];
+                }
+                if (gl == 0) cols[3 * N * G] = g ? cols[3 * N * G] + salpha : salpha;
+            }
+            __syncthreads();
+        }
+        if (threadIdx.x < G) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int j = column<G, VEC>(gl, i), k = gl + G * i;
+                if (j < q.W) { out[j] = cols[k]; out[q.W + j] = cols[N * G + k]; out[2 * q.W + j] = cols[2 * N * G + k]; }
+            }
+            if (gl == 0) out[3 * q.W] = cols[3 * N * G];
+        }
+    }
+}
+
+// the workgroups' sums added up: 64 columns by 4 parts of the workgroups, then the 4 parts
+struct Sums { const float* parts; int blocks, W; float* dpost; float* dpre; float* dgate; float* dalpha; };
+__global__ void __launch_bounds__(256) norm_sums_kernel(Sums q) {
+    __shared__ float lds[256];
+    const int C = 3 * q.W + 1, col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    float v = 0.f;
+    if (col < C) {
+        const int b0 = (int)((long)q.blocks * part / 4), b1 = (int)((long)q.blocks * (part + 1) / 4);
+#pragma unroll 8
+        for (int b = b0; b < b1; b++) v += q.parts[(long)b * C + col];
+    }
+    lds[threadIdx.x] = v;
+    __syncthreads();
+    if (part || col >= C) return;
+    v = (lds[threadIdx.x] + lds[threadIdx.x + 64]) + (lds[threadIdx.x + 128] + lds[threadIdx.x + 192]);
+    float* to = col < q.W ? q.dpost : col < 2 * q.W ? q.dpre : col < 3 * q.W ? q.dgate : q.dalpha;
+    if (to) to[col < 3 * q.W ? col % q.W : 0] = v;
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------------------
+int lanes_of(int W) { return W <= 16 * N ? 16 : W <= 64 * N ? 64 : W <= 256 * N ? 256 : 1024; }
+// workgroups of the backward pass: each leaves 3 W + 1 sums, so no more than keep the chip full
+int blocks_of(long R, int W) {
+    const int G = lanes_of(W), rows = G > 256 ? 1 : 256 / G;
+    const long need = (R + rows - 1) / rows, most = G > 256 ? 512 : 1024;
+    return (int)(need < most ? need : most);
+}
+bool aligned(const void* p, long stride, int size) { return !p || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * size) % 16 == 0); }
+
+template <typename TX, typename TY, int G, int VEC> int go(const Norm& q, bool grad, hipStream_t s) {
+    constexpr int T = G > 256 ? G : 256, ROWS = T / G;
+    if (grad) hipLaunchKernelGGL((norm_grad_kernel<TX, TY, G, VEC>), dim3((unsigned)blocks_of(q.R, q.W)), dim3(T), 0, s, q);
+    else {
+        const long need = (q.R + ROWS - 1) / ROWS;
+        hipLaunchKernelGGL((norm_kernel<TX, TY, G, VEC>), dim3((unsigned)(need < 2048 ? need : 2048)), dim3(T), 0, s, q);
+    }
+    return check_launch();
+}
+template <typename TX, typename TY, int VEC> int by_lanes(const Norm& q, bool grad, hipStream_t s) {
+    switch (lanes_of(q.W)) {
+        case 16: return go<TX, TY, 16, VEC>(q, grad, s);
+        case 64: return go<TX, TY, 64, VEC>(q, grad, s);
+        case 256: return go<TX, TY, 256, VEC>(q, grad, s);
+        default: return go<TX, TY, 1024, VEC>(q, grad, s);
+    }
+}
+template <typename TX, typename TY> int by_vec(const Norm& q, bool grad, hipStream_t s) {
+    const int sx = sizeof(TX), sy = sizeof(TY);
+    bool v = q.W % 8 == 0 && aligned(q.x, q.xs, sx) && aligned(q.y, q.ys, sy) && aligned(q.post, 0, 4) && aligned(q.pre, 0, 4);
+    if (q.kind == BL_GATE_FULL) v = v && aligned(q.gate, q.gs, sy) && aligned(q.dgate, q.dgs, sy);
+    if (q.kind == BL_GATE_CHANNEL) v = v && aligned(q.gate, 0, 4);
+    v = v && aligned(q.xo, q.W, sx) && aligned(q.h, q.W, sy) && aligned(q.gx, q.gxs, sx) && aligned(q.gh, q.ghs, sy) && aligned(q.dx, q.W, sx) && aligned(q.dy, q.dys, sy);
+    return v ? by_lanes<TX, TY, 8>(q, grad, s) : by_lanes<TX, TY, 1>(q, grad, s);
+}
+int by_type(const Norm& q, int tx, int ty, bool grad, hipStream_t s) {
+    if (tx == BL_F32 && ty == BL_F32) return by_vec<float, float>(q, grad, s);
+    if (tx == BL_F32 && ty == BL_F16) return by_vec<float, f16>(q, grad, s);
+    if (tx == BL_F32 && ty == BL_BF16) return by_vec<float, bf16>(q, grad, s);
+    if (tx == BL_F16 && ty == BL_F16) return by_vec<f16, f16>(q, grad, s);
+    if (tx == BL_BF16 && ty == BL_BF16) return by_vec<bf16, bf16>(q, grad, s);
+    return BL_EINVAL;
+}
+int check_norm(const Norm& q) {
+    if (!q.x || q.R <= 0 || q.W <= 0 || !(q.eps >= 0.f) || q.xs < 0 || q.ys < 0 || q.gs < 0) return BL_EINVAL;
+    if (q.kind < BL_GATE_NONE || q.kind > BL_GATE_ROW || (q.kind != BL_GATE_NONE) != (q.gate != nullptr)) return BL_EINVAL;
+    if (!q.y && (q.kind != BL_GATE_NONE || q.post || !q.pre)) return BL_EINVAL;
+    return q.W > BL_NORM_MAX ? BL_ETOOBIG : BL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bl_norm_residual(const void* x, int x_dtype, long x_stride, const void* y, int y_dtype, long y_stride, const float* alpha,
+                     const float* post, const void* gate, int gate_kind, long gate_stride, const float* pre, float eps, long R, int W,
+                     void* x_out, void* h, float* stats, bl_stream_t stream) {
+    Norm q{};
+    q.x = x; q.xs = x_stride; q.y = y; q.ys = y_stride; q.alpha = alpha; q.post = post; q.gate = gate; q.gs = gate_stride; q.kind = gate_kind;
+    q.pre = pre; q.eps = eps; q.inv_w = 1.f / (float)W; q.R = R; q.W = W; q.xo = x_out; q.h = h; q.stats = stats;
+    if (const int rc = check_norm(q)) return rc;
+    if ((y != nullptr) != (x_out != nullptr) || (pre != nullptr) != (h != nullptr)) return BL_EINVAL;
+    return by_type(q, x_dtype, y_dtype, false, (hipStream_t)stream);
+}
+
+long bl_norm_residual_workspace(long R, int W) { return R <= 0 || W <= 0 || W > BL_NORM_MAX ? 0 : 4l * blocks_of(R, W) * (3l * W + 1); }
+
+int bl_norm_residual_grad(const void* x, int x_dtype, long x_stride, const void* y, int y_dtype, long y_stride, const float* alpha,
+                          const float* post, const void* gate, int gate_kind, long gate_stride, const float* pre, float eps, long R,
+                          int W, const float* stats, const void* g_x, long g_x_stride, const void* g_h, long g_h_stride, void* d_x,
+                          void* d_y, long d_y_stride, void* d_gate, long d_gate_stride, float* d_alpha, float* d_post, float* d_pre,
+                          void* workspace, bl_stream_t stream) {
+    Norm q{};
+    q.x = x; q.xs = x_stride; q.y = y; q.ys = y_stride; q.alpha = alpha; q.post = post; q.gate = gate; q.gs = gate_stride; q.kind = gate_kind;
+    q.pre = pre; q.eps = eps; q.inv_w = 1.f / (float)W; q.R = R; q.W = W; q.stats = (float*)stats;
+    q.gx = g_x; q.gxs = g_x_stride; q.gh = g_h; q.ghs = g_h_stride; q.dx = d_x; q.dy = d_y; q.dys = d_y_stride;
+    q.dgate = gate_kind == BL_GATE_CHANNEL ? nullptr : d_gate; q.dgs = d_gate_stride; q.parts = (float*)workspace;
+    if (const int rc = check_norm(q)) return rc;
+    if (!stats || !d_x || !workspace || (y != nullptr) != (d_y != nullptr) || (g_h && !pre) || g_x_stride < 0 || g_h_stride < 0 || d_y_stride < 0 || d_gate_stride < 0) return BL_EINVAL;
+    if (const int rc = by_type(q, x_dtype, y_dtype, true, (hipStream_t)stream)) return rc;
+    if (!d_alpha && !d_post && !d_pre && !(gate_kind == BL_GATE_CHANNEL && d_gate)) return BL_OK;
+    Sums t{q.parts, blocks_of(R, W), W, d_post, d_pre, gate_kind == BL_GATE_CHANNEL ? (float*)d_gate : nullptr, d_alpha};
+    hipLaunchKernelGGL(norm_sums_kernel, dim3((unsigned)((3 * W + 1 + 63) / 64)), dim3(256), 0, (hipStream_t)stream, t);
+    return check_launch();
+}
+
+}  // extern "C"

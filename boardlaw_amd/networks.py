@@ -3,9 +3,10 @@ fully-connected residual blocks, masked log-softmax policy head and tanh value h
 (state_dict keys identical to the reference's: body.N.weight/bias/α, policy.core.*, value.core.*)."""
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
-from . import arrdict, heads
+from . import _native, arrdict, heads
 
 
 class ReZeroResidual(nn.Linear):
@@ -20,14 +21,175 @@ class ReZeroResidual(nn.Linear):
         return x + getattr(self, 'α') * super().forward(F.relu(x))
 
 
-class FCModel(nn.Module):
+GATES = {'none': 0, 'full': 1, 'channel': 2, 'row': 3}          # BL_GATE_*
 
-    def __init__(self, obs_space, action_space, width=256, depth=64):
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _norm_args(x, y, alpha, post, gate, kind, pre, eps, h_dtype):
+    """The leading arguments of bl_norm_residual and its gradient: x (R,W); y (R,W), or (R,2W) holding the gate behind the values (kind 'packed')."""
+    R, W = x.shape
+    if kind == 'packed':
+        g, gs, code = y.data_ptr() + W * y.element_size(), y.stride(0), GATES['full']
+    else:
+        g, gs, code = _ptr(gate), gate.stride(0) if kind in ('full', 'row') else 0, GATES[kind]
+    return (x.data_ptr(), _native.DTYPES[x.dtype], x.stride(0), _ptr(y), _native.DTYPES[h_dtype], 0 if y is None else y.stride(0), _ptr(alpha),
+            _ptr(post), g, code, gs, _ptr(pre), eps, R, W)
+
+
+def _norm_residual(x, y, alpha, post, gate, kind, pre, eps, h_dtype, want_stats):
+    R, W = x.shape
+    new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=x.device)
+    out = new(x.dtype, R, W) if y is not None else None
+    h = new(h_dtype, R, W) if pre is not None else None
+    stats = new(torch.float32, R, 2) if want_stats else None
+    if R:
+        with _native.on(x.device):
+            _native.check(_native.lib().bl_norm_residual(*_norm_args(x, y, alpha, post, gate, kind, pre, eps, h_dtype), _ptr(out), _ptr(h), _ptr(stats),
+                                                         _native.stream(x.device)))
+    return out, h, stats
+
+
+class _NormResidual(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, y, alpha, post, gate, pre, kind, eps, h_dtype):
+        out, h, stats = _norm_residual(x, y, alpha, post, gate, kind, pre, eps, h_dtype, True)
+        ctx.save_for_backward(x, y, alpha, post, gate, pre, stats)
+        ctx.kind, ctx.eps, ctx.h_dtype = kind, eps, h_dtype
+        ctx.set_materialize_grads(False)
+        return out, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_out, g_h):
+        x, y, alpha, post, gate, pre, stats = ctx.saved_tensors
+        R, W = x.shape
+        new = lambda like: None if like is None else torch.empty(like.shape, dtype=like.dtype, device=x.device)
+        dx, dy, dalpha, dpost, dgate = (new(t) for t in (x, y, alpha, post, gate))
+        dpre = new(pre) if g_h is not None else None
+        if R == 0:
+            return (dx, dy) + tuple(None if t is None else t.zero_() for t in (dalpha, dpost, dgate, dpre)) + (None,) * 3
+        g_out, g_h = (None if g is None else _native.rows_of(g, W) for g in (g_out, g_h))
+        if ctx.kind == 'packed':
+            dg, dgs = dy.data_ptr() + W * dy.element_size(), dy.stride(0)
+        else:
+            dg, dgs = _ptr(dgate), dgate.stride(0) if ctx.kind in ('full', 'row') else 0
+        L = _native.lib()
+        work = torch.empty(L.bl_norm_residual_workspace(R, W), dtype=torch.uint8, device=x.device)
+        with _native.on(x.device):
+            _native.check(L.bl_norm_residual_grad(
+                *_norm_args(x, y, alpha, post, gate, ctx.kind, pre, ctx.eps, ctx.h_dtype), stats.data_ptr(),
+                _ptr(g_out), 0 if g_out is None else g_out.stride(0), _ptr(g_h), 0 if g_h is None else g_h.stride(0),
+                dx.data_ptr(), _ptr(dy), 0 if dy is None else dy.stride(0), dg, dgs, _ptr(dalpha), _ptr(dpost), _ptr(dpre),
+                work.data_ptr(), _native.stream(x.device)))
+        return dx, dy, dalpha, dpost, dgate, dpre, None, None, None
+
+
+def norm_residual(x, y=None, alpha=None, post=None, gate=None, pre=None, eps=1e-5, dtype=None):
+    """The residual stream between two blocks in one pass -- norm behind the block, its gate, the residual scale, norm before the next block:
+
+        n = post * y / rms(y)            (post None: n = y)
+        x_out = x + alpha * sigmoid(gate) * n
+        h = pre * x_out / rms(x_out)     rms(v) = sqrt(mean(v ** 2, -1) + eps)
+
+        x      (..., W) f32 / f16 / bf16, W up to 8192
+        y      (..., W) the block's output, of x's type, or f16 / bf16 beside an f32 stream; or (..., 2W): values, then their gates, as one
+               Linear makes them.  None: only h.
+        alpha  f32 scalar tensor, None: 1.  post, pre (W,) f32 gains; pre None: no h
+        gate   what goes through the sigmoid: (..., W) or (..., 1) of y's type, or (W,) f32, one per channel (for a one-dimensional x: of the channel)
+        dtype  h's type where y is None (default: x's); else it is y's
+
+    -> (x_out, h).  Computed in f32, each result rounded once; differentiable (once) in every tensor.  On the GPU only (bl_norm_residual)."""
+    if x.dtype not in _native.DTYPES:
+        raise TypeError(f'x must be float32, float16 or bfloat16, got {x.dtype}')
+    if x.ndim < 1 or not 1 <= x.shape[-1] <= _native.NORM_MAX:
+        raise ValueError(f'x must be (..., W) with W in 1 .. {_native.NORM_MAX}, got {tuple(x.shape)}')
+    lead, W = x.shape[:-1], x.shape[-1]
+    _native.require_device(*(t for t in (x, y, alpha, post, gate, pre) if t is not None))
+    if y is None:
+        if alpha is not None or post is not None or gate is not None or pre is None:
+            raise ValueError('without y there is only h = pre * x / rms(x): alpha, post and gate must be None and pre given')
+    elif y.shape[:-1] != lead or y.shape[-1] not in (W, 2 * W):
+        raise ValueError(f'y must be {(*lead, W)} or {(*lead, 2 * W)}, got {tuple(y.shape)}')
+    h_dtype = y.dtype if y is not None else (dtype or x.dtype)
+    if h_dtype != x.dtype and not (x.dtype == torch.float32 and h_dtype in _native.DTYPES):
+        raise TypeError(f"y (or dtype) must be of x's type, or float16 / bfloat16 beside float32: got {x.dtype} and {h_dtype}")
+    if y is not None and dtype not in (None, y.dtype):
+        raise TypeError("h is of y's type")
+    for name, t, shape in (('alpha', alpha, ()), ('post', post, (W,)), ('pre', pre, (W,))):
+        if t is not None and (t.shape != shape or t.dtype != torch.float32):
+            raise ValueError(f'{name} must be float32 of shape {shape}, got {t.dtype} {tuple(t.shape)}')
+    if not eps >= 0:
+        raise ValueError(f'eps must not be negative, got {eps}')
+    kind = 'none'
+    if y is not None and y.shape[-1] == 2 * W:
+        kind = 'packed'
+        if gate is not None:
+            raise ValueError('y holds the gates already')
+    elif gate is not None:
+        kind = 'channel' if gate.shape == (W,) else 'full' if gate.shape == x.shape else 'row' if gate.shape == (*lead, 1) else None
+        if kind is None:
+            raise ValueError(f'gate must be {(W,)}, {tuple(x.shape)} or {(*lead, 1)}, got {tuple(gate.shape)}')
+        if gate.dtype != (torch.float32 if kind == 'channel' else h_dtype):
+            raise TypeError(f"a gate per channel is float32, any other of y's type: got {gate.dtype}")
+    flat = lambda t, w: None if t is None else _native.rows_of(t, w)
+    solid = lambda t: None if t is None else t.contiguous()
+    xs, ys = flat(x, W), flat(y, y.shape[-1] if y is not None else 0)
+    gs = solid(gate) if kind == 'channel' else flat(gate, gate.shape[-1]) if gate is not None else None
+    tensors = (xs, ys, alpha, solid(post), gs, solid(pre))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        out, h = _NormResidual.apply(*tensors, kind, eps, h_dtype)
+    else:
+        out, h, _ = _norm_residual(tensors[0], tensors[1], alpha, tensors[3], gs, kind, tensors[5], eps, h_dtype, False)
+    return (x if out is None else out.view(x.shape)), (None if h is None else h.view(x.shape))
+
+
+class GatedResidual(nn.Linear):
+    """A block of the gated network: x + α * sigmoid(g) * post * v / rms(v), (v, g) = Linear(pre * x / rms(x)), α initialised to 0 like
+    ReZeroResidual's.  GatedStack runs the blocks: what is behind one Linear and before the next is one norm_residual."""
+
+    def __init__(self, width):
+        super().__init__(width, 2 * width)
+        nn.init.orthogonal_(self.weight[:width].detach())
+        nn.init.orthogonal_(self.weight[width:].detach())
+        self.register_parameter('α', nn.Parameter(torch.zeros(())))
+        self.pre, self.post = nn.Parameter(torch.ones(width)), nn.Parameter(torch.ones(width))
+
+
+class GatedStack(nn.Sequential):
+    """An intake and GatedResidual blocks.  The stream is f32, also under autocast; the branches are what the Linears make."""
+
+    def forward(self, obs):
+        intake, *blocks = self
+        dtype = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else torch.float32
+        return run_gated(intake(obs).float(), blocks, [(b.weight, b.bias) for b in blocks], dtype)
+
+
+def run_gated(x, blocks, linears, dtype):
+    """The stream through GatedResidual blocks, the Linears' weights given (a plan's casts, or the blocks' own)."""
+    h = None
+    if blocks:
+        _, h = norm_residual(x, pre=blocks[0].pre, dtype=dtype)
+    for i, (block, (weight, bias)) in enumerate(zip(blocks, linears)):
+        x, h = norm_residual(x, F.linear(h, weight, bias), getattr(block, 'α'), block.post, pre=blocks[i + 1].pre if i + 1 < len(blocks) else None)
+    return x
+
+
+class FCModel(nn.Module):
+    """block: 'rezero', the reference's residual blocks, or 'gated' (GatedResidual: normed and gated; on the GPU only)."""
+
+    def __init__(self, obs_space, action_space, width=256, depth=64, block='rezero'):
+        if block not in ('rezero', 'gated'):
+            raise ValueError(f"block must be 'rezero' or 'gated', got {block!r}")
         super().__init__()
         self.obs_space, self.action_space = obs_space, action_space
         self.policy = heads.output(action_space, width)
         self.sampler = self.policy.sample
-        self.body = nn.Sequential(heads.intake(obs_space, width), *[ReZeroResidual(width) for _ in range(depth)])
+        stack, make = (nn.Sequential, ReZeroResidual) if block == 'rezero' else (GatedStack, GatedResidual)
+        self.body = stack(heads.intake(obs_space, width), *[make(width) for _ in range(depth)])
         self.value = heads.ValueOutput(width)
 
     def forward(self, worlds):
@@ -134,8 +296,13 @@ class Inference:
         srcs += [m.policy.core.weight, m.policy.core.bias, m.value.core.weight, m.value.core.bias]
         return srcs, [getattr(blk, 'α') for blk in blocks[1:]]
 
+    def _gated(self):
+        return isinstance(self.model.body, GatedStack)
+
     def _fusable(self):
         m = self.model
+        if self._gated():
+            return False
         blocks = list(m.body)
         W, K0 = blocks[0].weight.shape
         A = m.policy.core.weight.shape[0]
@@ -148,6 +315,8 @@ class Inference:
         """bl_root_mlp_f32's limits: fp32 parameters on the GPU, width a multiple of 128 up to 1024, the flattened
         observation no wider than the body."""
         m = self.model
+        if self._gated():
+            return False
         blocks = list(m.body)
         W, K0 = blocks[0].weight.shape
         return (W % 128 == 0 and 128 <= W <= 1024 and -(-K0 // 64) * 64 <= W and blocks[0].weight.dtype == torch.float
@@ -267,6 +436,9 @@ class Inference:
             return policy, value
         with torch.no_grad():
             x = F.linear(x0, blocks[0].weight, blocks[0].bias)
+            if self._gated():
+                x = run_gated(x, blocks[1:], [(b.weight, b.bias) for b in blocks[1:]], torch.float32)
+                blocks = blocks[:1]
             r = F.relu(x)
             for blk in blocks[1:]:
                 y = F.linear(r, blk.weight, blk.bias)
@@ -365,6 +537,11 @@ class Inference:
                 _native.check(rc)
             return policy, value
         x = F.linear(x0, w[0], w[1])
+        if self._gated():
+            blocks = list(self.model.body)[1:]
+            with torch.no_grad():
+                x = run_gated(x.float(), blocks, [(w[2 + 2 * i], w[3 + 2 * i]) for i in range(len(blocks))], torch.half).half()
+            alphas = []
         r = F.relu(x)
         for i, alpha in enumerate(alphas):
             y = F.linear(r, w[2 + 2 * i], w[3 + 2 * i])

@@ -1,0 +1,118 @@
+"""The learner's optimiser for hidden weights: momentum updates orthogonalised by Newton-Schulz products before they are applied.  The
+reference trains with Adam alone (boardlaw/main.py:153); here `training.run(optimizer='muon')` gives the residual blocks' weights
+to Muon and everything else to Adam."""
+import ctypes
+
+import torch
+
+from . import _native, networks
+
+
+def _orthogonalize(mats, steps, eps):
+    """Matrices of one shape, type and device -> contiguous results."""
+    rows, cols = mats[0].shape
+    dev, count = mats[0].device, len(mats)
+    mats = [m.detach().contiguous() for m in mats]
+    # results in one allocation, each matrix on a 16-byte boundary or better
+    size = rows * cols * mats[0].element_size()
+    pitch = -(-size // 16) * 16 // mats[0].element_size()
+    outs = [o[:rows * cols].view(rows, cols) for o in torch.empty((count, pitch), dtype=mats[0].dtype, device=dev).unbind(0)]
+    L = _native.lib()
+    work = torch.empty(L.bl_orthogonalize_workspace(count, rows, cols), dtype=torch.uint8, device=dev)
+    pointers = ctypes.c_void_p * count
+    with _native.on(dev):
+        _native.check(L.bl_orthogonalize(pointers(*[m.data_ptr() for m in mats]), pointers(*[o.data_ptr() for o in outs]), count,
+                                         _native.DTYPES[mats[0].dtype], rows, cols, steps, eps, work.data_ptr(), _native.stream(dev)))
+    return outs
+
+
+def orthogonalize(matrices, steps=5, eps=1e-7):
+    """The Newton-Schulz iteration X = aX + (bA + cA^2)X, A = XX^T, from X = G / (|G| + eps): the matrix with G's singular vectors and singular
+    values near 1 (0.7 .. 1.2 after five steps; those under about 1e-3 of |G| have not got there yet).
+
+        matrices  a tensor (..., m, n), or a list of matrices (m, n) of any shapes: f32, f16 or bf16, sides up to 16384
+
+    -> the same structure, types and shapes; f32 sums and 22-bit operands whatever the type.  Matrices of one shape and type are taken
+    through it together.  Not differentiable.  On the GPU only (bl_orthogonalize)."""
+    if not isinstance(steps, int) or steps < 1:
+        raise ValueError(f'steps must be a whole number from 1 on, got {steps!r}')
+    if not eps >= 0:
+        raise ValueError(f'eps must not be negative, got {eps}')
+    if isinstance(matrices, torch.Tensor):
+        if matrices.ndim < 2:
+            raise ValueError(f'a matrix or a batch of them is wanted, got {tuple(matrices.shape)}')
+        flat = matrices.reshape(-1, *matrices.shape[-2:])
+        if flat.numel() == 0:
+            _native.require_device(matrices)
+            return torch.empty_like(matrices)
+        return torch.stack(orthogonalize(list(flat.unbind(0)), steps, eps)).view(matrices.shape)
+    groups, outs = {}, [None] * len(matrices)
+    for i, m in enumerate(matrices):
+        if m.dtype not in _native.DTYPES:
+            raise TypeError(f'matrices must be float32, float16 or bfloat16, got {m.dtype}')
+        if m.ndim != 2:
+            raise ValueError(f'matrices must be two-dimensional, got {tuple(m.shape)}')
+        if max(m.shape) > _native.ORTHO_MAX:
+            raise ValueError(f'sides up to {_native.ORTHO_MAX} are supported, got {tuple(m.shape)}')
+        _native.require_device(m)
+        if m.numel() == 0:
+            outs[i] = torch.empty_like(m)
+        else:
+            groups.setdefault((m.shape, m.dtype, m.device), []).append(i)
+    for members in groups.values():
+        for i, o in zip(members, _orthogonalize([matrices[i] for i in members], steps, eps)):
+            outs[i] = o
+    return outs
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum SGD whose update of every weight matrix is orthogonalised: m = momentum m + g, u = g + momentum m (nesterov) or m,
+    W = (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) orthogonalize(u).  For the two-dimensional weights of hidden layers."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0., steps=5):
+        if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0:
+            raise ValueError(f'lr and weight_decay must not be negative, momentum in [0, 1): got {lr}, {weight_decay}, {momentum}')
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
+        for group in self.param_groups:
+            for p in group['params']:
+                if p.ndim != 2:
+                    raise ValueError(f'Muon is for matrices, got a parameter of shape {tuple(p.shape)}')
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group['params'] if p.grad is not None]
+            if not params:
+                continue
+            grads = [p.grad for p in params]
+            moments = []
+            for p in params:
+                state = self.state[p]
+                if 'momentum' not in state:
+                    state['momentum'] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                moments.append(state['momentum'])
+            torch._foreach_mul_(moments, group['momentum'])
+            torch._foreach_add_(moments, grads)
+            updates = torch._foreach_add(grads, moments, alpha=group['momentum']) if group['nesterov'] else moments
+            updates = orthogonalize(updates, steps=group['steps'])
+            if group['weight_decay']:
+                torch._foreach_mul_(params, 1 - group['lr'] * group['weight_decay'])
+            scales = {}
+            for p, u in zip(params, updates):
+                ps, us = scales.setdefault(max(1., p.shape[0] / p.shape[1]) ** .5, ([], []))
+                ps.append(p); us.append(u)
+            for scale, (ps, us) in scales.items():
+                torch._foreach_add_(ps, us, alpha=-group['lr'] * scale)
+        return loss
+
+
+def split(network):
+    """A network's parameters as (hidden weight matrices, the rest): the residual blocks' weights are Muon's, biases, gains, the intake
+    and the heads Adam's."""
+    hidden = [m.weight for m in network.modules() if isinstance(m, (networks.ReZeroResidual, networks.GatedResidual))]
+    ids = {id(p) for p in hidden}
+    return hidden, [p for p in network.parameters() if id(p) not in ids]

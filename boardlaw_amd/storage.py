@@ -75,7 +75,8 @@ def network_from_state(agent_state, device='cpu'):
     if boardsize * boardsize != cells or n_inputs != 2 * cells:
         raise ValueError(f'Not a Hex FCModel: {cells} actions, {n_inputs} inputs')
     depth = sum(1 for k in sd if k.startswith('body.') and k.endswith('.α'))
-    net = networks.FCModel(heads.Tensor((boardsize, boardsize, 2)), heads.Masked(cells), width=width, depth=depth)
+    net = networks.FCModel(heads.Tensor((boardsize, boardsize, 2)), heads.Masked(cells), width=width, depth=depth,
+                           block='gated' if 'body.1.post' in sd else 'rezero')
     net.load_state_dict(sd, strict=True)
     return net.to(device)
 

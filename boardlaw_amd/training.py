@@ -11,7 +11,7 @@ import time
 import numpy as np
 import torch
 
-from . import arrdict, learning, parallel
+from . import arrdict, heads, learning, parallel
 
 
 def _sync(dev):
@@ -30,45 +30,67 @@ def as_chunk(buffer, batch_size):
     return chunk, buffer[n_new:]
 
 
-def losses(network, batch):
-    """Policy cross-entropy against the search's root distribution + value MSE against reward-to-go (main.py:78-92)."""
+def losses(network, batch, entropy=0.):
+    """Policy cross-entropy against the search's root distribution + value MSE against reward-to-go (main.py:78-92).
+    entropy: the weight of an entropy bonus, taken off the policy loss (heads.logprobs; the reference has none)."""
     d0 = batch.decisions
     d = network(batch.worlds)
     zeros = torch.zeros_like(d.logits)
     l = d.logits.where(d.logits > -np.inf, zeros)
     l0 = d0.logits.float().where(d0.logits > -np.inf, zeros.float())
     policy_loss = -(l0.exp() * l).sum(-1).mean()
+    if entropy:
+        policy_loss = policy_loss - entropy * heads.logprobs(d.logits).entropy.mean()
     value_loss = (batch.reward_to_go - d.v).square().mean()
     return policy_loss, value_loss
 
 
-def optimize(network, scaler, opt, batch, sync_gradients=True, bucket=None):
+def optimize(network, scaler, opt, batch, sync_gradients=True, bucket=None, entropy=0.):
     """One learner step (main.py:76-98).  Returns (policy_loss, value_loss) as detached tensors.
+    opt: an optimiser, or several that share the network's parameters out among them.  entropy: see losses().
     bucket: a parallel.GradientBucket over `network` -- the gradients then live in one flat buffer that is zeroed, accumulated
     into, all-reduced and read by the optimiser in place (what `run` uses when there are several ranks)."""
     cuda = next(network.parameters()).is_cuda
+    opts = opt if isinstance(opt, (list, tuple)) else (opt,)
     with torch.autocast('cuda', enabled=cuda):
-        policy_loss, value_loss = losses(network, batch)
+        policy_loss, value_loss = losses(network, batch, entropy)
         loss = policy_loss + value_loss
     if bucket is not None:
         bucket.zero()
     else:
-        opt.zero_grad()
+        for o in opts:
+            o.zero_grad()
     scaler.scale(loss).backward()
     if sync_gradients:
         if bucket is not None:
             bucket.allreduce()
         else:
             parallel.allreduce_gradients(network)
-    scaler.step(opt)
+    for o in opts:
+        scaler.step(o)
     scaler.update()
     return policy_loss.detach(), value_loss.detach()
 
 
-def run(worlds, network, n_steps, nodes=64, c_puct=1 / 16, lr=1e-3, buffer_len=64, graph=False, inference=None, on_step=None, timings=None):
+def make_optimizer(network, optimizer='adam', lr=1e-3, hidden_lr=0.02):
+    """What run() trains with: 'adam' as main.py:153, or 'muon': optim.Muon for the residual blocks' weights and Adam for the rest."""
+    if optimizer == 'adam':
+        return torch.optim.Adam(network.parameters(), lr=lr)
+    if optimizer != 'muon':
+        raise ValueError(f"optimizer must be 'adam' or 'muon', got {optimizer!r}")
+    from . import optim
+    hidden, rest = optim.split(network)
+    if not hidden:
+        raise ValueError('the network has no residual blocks for Muon')
+    return optim.Muon(hidden, lr=hidden_lr), torch.optim.Adam(rest, lr=lr)
+
+
+def run(worlds, network, n_steps, nodes=64, c_puct=1 / 16, lr=1e-3, buffer_len=64, graph=False, inference=None, on_step=None, timings=None,
+        optimizer='adam', hidden_lr=0.02, entropy=0.):
     """main.py:147-200 minus run bookkeeping.  `worlds` is this rank's env shard.  Returns the final worlds.
     inference: None (the module under autocast, as the reference), 'torch' or 'fused' (networks.Inference plans; their
     f16 weights are refreshed from the module at the start of every move, so optimiser steps are seen).
+    optimizer, hidden_lr: see make_optimizer; entropy: the weight of an entropy bonus (losses).
 
     `worlds` may also be a list of independent env batches -- several ACTORS on this GPU sharing the network.  Each actor
     searches on its own stream with its own generator (the search kernels are latency-bound, so a second resident search
@@ -90,7 +112,7 @@ def run(worlds, network, n_steps, nodes=64, c_puct=1 / 16, lr=1e-3, buffer_len=6
             kwargs['rng'] = MoveRng(generator=gen)
             streams.append(torch.cuda.Stream(device=dev))
         agents.append(MCTSAgent(actor, n_nodes=nodes, c_puct=c_puct, graph=graph, **kwargs))
-    opt = torch.optim.Adam(network.parameters(), lr=lr)
+    opt = make_optimizer(network, optimizer, lr, hidden_lr)
     scaler = torch.amp.GradScaler('cuda', enabled=(dev.type == 'cuda'))
     # several ranks: the gradients live in one flat buffer that is all-reduced where it lies (parallel.GradientBucket)
     # (built ONCE; under the benchmark the same code path runs in a one-rank group, too, every collective bracketed by device events)
@@ -143,7 +165,7 @@ def run(worlds, network, n_steps, nodes=64, c_puct=1 / 16, lr=1e-3, buffer_len=6
             if timings is not None:
                 _sync(dev); t0 = time.perf_counter()
             chunk, buffers[i] = as_chunk(buffers[i], batches[i].n_envs)
-            pl, vl = optimize(network, scaler, opt, chunk[idxs[i]], bucket=bucket)
+            pl, vl = optimize(network, scaler, opt, chunk[idxs[i]], bucket=bucket, entropy=entropy)
             if timings is not None:
                 _sync(dev); timings.setdefault('learner_s', []).append(time.perf_counter() - t0)
             if on_step is not None:

@@ -403,6 +403,72 @@ int bl_sim_expand_counted(const bl_search_t* s, int sim, const void* rands, int1
                           uint8_t* valid_out, int32_t* leaf_seats_out, unsigned long long* counters,
                           bl_stream_t stream);
 
+/* ================= operators of the learner's step (no reference counterpart) =====================================
+ * Element types of the tensors below: f32, f16, bf16.  Row strides are in elements; the last dimension is contiguous. */
+#define BL_F32 0
+#define BL_F16 1
+#define BL_BF16 2
+
+/* Log probabilities of given moves, entropy and the best alternatives of R rows of A unnormalised logits (A <= 2^30, R <= 2^24).
+ * valid (R,A) u8 or NULL: entries with 0 count as logits of -inf, whatever raw holds there; an entry of -inf has probability 0, is never an
+ * alternative, and its gradient is 0.  Per row, with log p = log_softmax:
+ *   logp_out[r] = log p[actions[r]]: -inf for an entry of probability 0; 0 if actions[r] < 0 (no move given); NaN if actions[r] >= A.
+ *     actions NULL: logp_out NULL.
+ *   entropy_out[r] = -sum p log p.
+ *   top_out / top_logp_out (R,k), k <= BL_TOP_MAX: the k best entries in descending order, equal ones by index, and their log p; -1 and -inf
+ *     where fewer than k have a probability.
+ *   stats_out (R,2) or NULL: what the gradient call reads.
+ * A row without valid entries has entropy 0 and no alternatives.  A NaN or +inf among the valid entries makes the row's numbers NaN (NaN is
+ * the best alternative).  workspace: bl_logprobs_workspace(R, A, k) bytes, 8-byte aligned (0: may be NULL).  All sums in f32, in an order
+ * that depends on the arguments only. */
+#define BL_TOP_MAX 64
+long bl_logprobs_workspace(long R, int A, int k);
+int bl_logprobs(const void* raw, int dtype, long raw_stride, const uint8_t* valid, long valid_stride, const long long* actions /*i64 (R)*/,
+                long R, int A, int k, float* logp_out /*(R)*/, float* entropy_out /*(R)*/, long long* top_out, float* top_logp_out,
+                float* stats_out, void* workspace, bl_stream_t stream);
+
+/* Its gradient: d_raw (R,A) contiguous, of raw's type, fully written, from the gradients of logp_out, entropy_out (R) and top_logp_out (R,k)
+ * (each may be NULL: zero).  entropy, top and stats are the forward call's outputs. */
+int bl_logprobs_grad(const void* raw, int dtype, long raw_stride, const uint8_t* valid, long valid_stride, const long long* actions, long R,
+                     int A, int k, const long long* top, const float* stats, const float* entropy, const float* g_logp,
+                     const float* g_entropy, const float* g_top, void* d_raw, bl_stream_t stream);
+
+/* The residual stream between two blocks of a pre- and post-normed network, R rows of W <= BL_NORM_MAX:
+ *     n = post y / rms(y)  (post NULL: n = y),  x_out = x + alpha sigmoid(gate) n,  h = pre x_out / rms(x_out),  rms(v) = sqrt(mean v^2 + eps)
+ * x, x_out of x_dtype, y and h of y_dtype: equal, or x f32 and y f16 / bf16.  alpha: one f32 on the device, NULL = 1.  post, pre (W) f32.
+ * gate by gate_kind: none (NULL); per element (R rows of W, y's type); per channel (W) f32; per row (one of y's type every gate_stride).
+ * y NULL (then no gate, no post, x_out NULL): h = pre x / rms(x) only.  pre NULL: no h.  x_out, h contiguous.
+ * stats_out (R,2) f32 or NULL: what the gradient call reads.  Computed in f32, each output rounded once. */
+#define BL_NORM_MAX 8192
+#define BL_GATE_NONE 0
+#define BL_GATE_FULL 1
+#define BL_GATE_CHANNEL 2
+#define BL_GATE_ROW 3
+int bl_norm_residual(const void* x, int x_dtype, long x_stride, const void* y, int y_dtype, long y_stride, const float* alpha,
+                     const float* post, const void* gate, int gate_kind, long gate_stride, const float* pre, float eps, long R, int W,
+                     void* x_out, void* h, float* stats_out, bl_stream_t stream);
+
+/* Its gradient from g_x (of x_out) and g_h (of h; either may be NULL: zero), given the forward call's inputs and stats.  d_x contiguous; d_y and
+ * a per-element d_gate with row strides (so that both can lie in one (R,2W) tensor); d_gate per row: one every d_gate_stride; per
+ * channel: (W) f32.  d_alpha (1), d_post, d_pre (W) f32.  d_gate, d_alpha, d_post, d_pre may be NULL; d_y may not where y is given.
+ * workspace: bl_norm_residual_workspace(R, W) bytes.  The sums over rows are made in a fixed order, without atomics. */
+long bl_norm_residual_workspace(long R, int W);
+int bl_norm_residual_grad(const void* x, int x_dtype, long x_stride, const void* y, int y_dtype, long y_stride, const float* alpha,
+                          const float* post, const void* gate, int gate_kind, long gate_stride, const float* pre, float eps, long R, int W,
+                          const float* stats, const void* g_x, long g_x_stride, const void* g_h, long g_h_stride, void* d_x, void* d_y,
+                          long d_y_stride, void* d_gate, long d_gate_stride, float* d_alpha, float* d_post, float* d_pre, void* workspace,
+                          bl_stream_t stream);
+
+/* Newton-Schulz orthogonalisation of `count` matrices of one shape (rows, cols <= BL_ORTHO_MAX): X = G / (|G|_F + eps), then `steps` times
+ * X = a X + (b A + c A^2) X with A = X X^T, (a, b, c) = (3.4445, -4.7750, 2.0315) -- singular values go to about 1 (0.7 .. 1.2 after five
+ * steps).  host_in / host_out: HOST arrays of device pointers to contiguous row-major matrices of dtype, read before the call returns; in and out may be the
+ * same.  Operands are held to 22 bits and summed in f32 whatever dtype; the result is rounded once.  A zero matrix gives zeros.
+ * workspace: bl_orthogonalize_workspace(count, rows, cols) bytes, 16-byte aligned, this call's own until its work on `stream` is done. */
+#define BL_ORTHO_MAX 16384
+long bl_orthogonalize_workspace(int count, int rows, int cols);
+int bl_orthogonalize(const void* const* host_in, void* const* host_out, int count, int dtype, int rows, int cols, int steps, float eps,
+                     void* workspace, bl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
