@@ -166,6 +166,23 @@ def philox_state(generator, increment):
     return int(out[0]) & (2 ** 64 - 1), int(out[1]) & (2 ** 64 - 1), int(out[2]), int(out[3])
 
 
+OPSLIBPATH = os.path.join(HERE, '_torchops.so')
+_ops = None
+
+
+def ops():
+    """The learner-step operators as functions of torch tensors (csrc/bl_torchops.cpp)."""
+    global _ops
+    if _ops is None:
+        lib()                                   # the library it is linked to, behind torch's HIP runtime
+        stamp = OPSLIBPATH + '.torch'
+        if not os.path.exists(OPSLIBPATH) or (os.path.exists(stamp) and open(stamp).read().strip() != torch.__version__):
+            raise NativeError(f'{OPSLIBPATH} is missing or was built for another torch than {torch.__version__}: run `python -m boardlaw_amd.build`')
+        from . import _torchops
+        _ops = _torchops
+    return _ops
+
+
 def check(rc):
     if rc != 0:
         raise NativeError(f'libboardlaw_amd: {lib().bl_strerror(rc).decode()} (code {rc})')
@@ -225,21 +242,6 @@ def copy_many(dsts, srcs):
 
 def ptr(t):
     return t.data_ptr()
-
-
-DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}        # BL_F32, BL_F16, BL_BF16
-TOP_MAX, NORM_MAX, ORTHO_MAX = 64, 8192, 16384
-
-
-def on(device):
-    """Context in which `device` is the current one."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def rows_of(t, width):
-    """`t` (..., width) as (rows, width) with a contiguous last dimension: a view where the layout allows one."""
-    t = t if t.ndim == 2 else t.reshape(-1, width)
-    return t if t.stride(1) == 1 or width == 1 else t.contiguous()
 
 
 def require_device(*tensors):

@@ -2,6 +2,7 @@
 
   libboardlaw_amd.so   HIP kernels + the C ABI (include/boardlaw_amd.h), hipcc --offload-arch=gfx950
   libbl_torchgen.so    host-only shim that reads torch's generator state (csrc/bl_torchgen.cpp), host compiler + torch headers
+  _torchops.so         host-only extension module: the learner-step operators on torch tensors, with their autograd nodes (csrc/bl_torchops.cpp)
 
 hipcc cross-compiles without a GPU, so this runs in the build container; the .so files then travel with the tree.  Every
 translation unit is compiled to its own object (in parallel, only when stale) and the objects are linked: touching one
@@ -23,6 +24,8 @@ OBJDIR = os.path.join(HERE, 'build')
 LIB = os.path.join(HERE, 'libboardlaw_amd.so')
 GEN_SRC = os.path.join(HERE, 'csrc', 'bl_torchgen.cpp')
 GEN_LIB = os.path.join(HERE, 'libbl_torchgen.so')
+OPS_SRC = os.path.join(HERE, 'csrc', 'bl_torchops.cpp')
+OPS_LIB = os.path.join(HERE, '_torchops.so')
 GEN_STAMP = GEN_LIB + '.torch'      # the torch version the shim was compiled against: it reads torch C++ objects by layout
 
 # -ffp-contract=off: the search kernels must round like the reference's CPU path (no FMA); see DESIGN.md.
@@ -45,14 +48,18 @@ def _newer(target, deps):
 def _torchgen_stale():
     """The shim touches c10::GeneratorImpl and at::PhiloxCudaState by layout, so a libbl_torchgen.so built against another torch
     is stale whatever its mtime: the version it was built for is kept in a stamp file beside it."""
-    if _newer(GEN_LIB, [GEN_SRC]) or not os.path.exists(GEN_STAMP):
+    return _shim_stale(GEN_LIB, GEN_SRC)
+
+
+def _shim_stale(lib, src):
+    if _newer(lib, [src, HEADERS[0]]) or not os.path.exists(lib + '.torch'):
         return True
     import torch
-    return open(GEN_STAMP).read().strip() != torch.__version__
+    return open(lib + '.torch').read().strip() != torch.__version__
 
 
 def stale():
-    return _newer(LIB, SOURCES + HEADERS + [os.path.abspath(__file__)]) or _torchgen_stale()
+    return _newer(LIB, SOURCES + HEADERS + [os.path.abspath(__file__)]) or _torchgen_stale() or _shim_stale(OPS_LIB, OPS_SRC)
 
 
 def _hipcc():
@@ -62,28 +69,39 @@ def _hipcc():
     return hipcc
 
 
-def build_torchgen(force=False, verbose=False):
-    if not force and not _torchgen_stale():
-        return GEN_LIB
+def _build_shim(lib, src, extra, verbose):
+    """A host-compiled library against torch's headers; the stamp beside it names the torch it is good for."""
     import torch
     t = os.path.dirname(torch.__file__)
     cxx = shutil.which('g++') or shutil.which('c++')
     cmd = [cxx, '-O2', '-std=c++17', '-fPIC', '-shared', '-w', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{t}/include', f'-I{t}/include/torch/csrc/api/include',
-           '-I/opt/rocm/include', GEN_SRC, '-o', GEN_LIB + '.tmp', f'-L{t}/lib', '-ltorch_hip', '-lc10_hip', '-lc10', '-ltorch_cpu',
-           f'-Wl,-rpath,{t}/lib']
+           '-I/opt/rocm/include', src, '-o', lib + '.tmp', f'-L{t}/lib', '-ltorch_hip', '-lc10_hip', '-lc10', '-ltorch_cpu'] + extra + [f'-Wl,-rpath,{t}/lib']
     if verbose:
         print(' '.join(cmd))
     subprocess.check_call(cmd)
-    os.replace(GEN_LIB + '.tmp', GEN_LIB)
-    with open(GEN_STAMP, 'w') as f:
+    os.replace(lib + '.tmp', lib)
+    with open(lib + '.torch', 'w') as f:
         f.write(torch.__version__)
-    return GEN_LIB
+    return lib
+
+
+def build_torchgen(force=False, verbose=False):
+    return _build_shim(GEN_LIB, GEN_SRC, [], verbose) if force or _torchgen_stale() else GEN_LIB
+
+
+def build_torchops(force=False, verbose=False):
+    """After build()'s library, which it is linked to and finds beside itself."""
+    import sysconfig
+    if not force and not _shim_stale(OPS_LIB, OPS_SRC):
+        return OPS_LIB
+    return _build_shim(OPS_LIB, OPS_SRC, ['-I' + sysconfig.get_paths()['include'], '-ltorch_python', '-ltorch', '-L' + HERE, '-lboardlaw_amd', '-Wl,-rpath,$ORIGIN'], verbose)
 
 
 def build(force=False, verbose=False):
     build_torchgen(force, verbose)
     if not force and not _newer(LIB, SOURCES + HEADERS + [os.path.abspath(__file__)]):
+        build_torchops(force, verbose)
         return LIB
     hipcc = _hipcc()
     os.makedirs(OBJDIR, exist_ok=True)
@@ -103,6 +121,7 @@ def build(force=False, verbose=False):
         print(' '.join(link))
     subprocess.check_call(link)
     os.replace(LIB + '.tmp', LIB)
+    build_torchops(force, verbose)
     return LIB
 
 

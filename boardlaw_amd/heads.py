@@ -7,7 +7,6 @@ from collections import namedtuple
 import numpy as np
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
 from . import _native, arrdict
@@ -49,53 +48,6 @@ def intake(space, width):
     return kinds[name](space, width)
 
 
-def _logprobs(raw, actions, valid, k, want_stats):
-    R, A = raw.shape
-    dev = raw.device
-    new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=dev)
-    logp = new(R) if actions is not None else None
-    entropy = new(R)
-    top, top_logp = (new(R, k, dtype=torch.int64), new(R, k)) if k else (None, None)
-    stats = new(R, 2) if want_stats else None
-    if R:
-        L = _native.lib()
-        size = L.bl_logprobs_workspace(R, A, k)
-        work = new(size, dtype=torch.uint8) if size else None
-        p = lambda t: None if t is None else t.data_ptr()
-        with _native.on(dev):
-            _native.check(L.bl_logprobs(raw.data_ptr(), _native.DTYPES[raw.dtype], raw.stride(0), p(valid), 0 if valid is None else valid.stride(0),
-                                        p(actions), R, A, k, p(logp), entropy.data_ptr(), p(top), p(top_logp), p(stats), p(work), _native.stream(dev)))
-    return logp, entropy, top, top_logp, stats
-
-
-class _LogProbs(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, raw, actions, valid, k):
-        logp, entropy, top, top_logp, stats = _logprobs(raw, actions, valid, k, True)
-        ctx.k = k
-        ctx.save_for_backward(raw, actions, valid, top, stats, entropy)
-        ctx.set_materialize_grads(False)
-        if top is not None:
-            ctx.mark_non_differentiable(top)
-        return logp, entropy, top, top_logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_logp, g_entropy, g_top, g_top_logp):
-        raw, actions, valid, top, stats, entropy = ctx.saved_tensors
-        R, A = raw.shape
-        d = torch.empty((R, A), dtype=raw.dtype, device=raw.device)
-        if R:
-            gs = [None if g is None else g.float().contiguous() for g in (g_logp, g_entropy, g_top_logp)]
-            p = lambda t: None if t is None else t.data_ptr()
-            with _native.on(raw.device):
-                _native.check(_native.lib().bl_logprobs_grad(
-                    raw.data_ptr(), _native.DTYPES[raw.dtype], raw.stride(0), p(valid), 0 if valid is None else valid.stride(0), p(actions), R, A, ctx.k,
-                    p(top), stats.data_ptr(), entropy.data_ptr(), p(gs[0]), p(gs[1]), p(gs[2]), d.data_ptr(), _native.stream(raw.device)))
-        return d, None, None, None
-
-
 def logprobs(raw, actions=None, valid=None, k=0):
     """Log probabilities of given moves, entropy and the best alternatives of policy rows, in one pass over the logits:
 
@@ -108,35 +60,13 @@ def logprobs(raw, actions=None, valid=None, k=0):
     in descending order, equal ones by index; where fewer than k moves are valid the rest is -1 and -inf.  An invalid given move
     has logp -inf, a missing one (-1) 0, one beyond the row NaN.  A row with no valid move has entropy 0.  Differentiable (once) in `raw` through
     logp, entropy and top_logp; an invalid move's gradient is 0.  On the GPU only (bl_logprobs)."""
-    if raw.dtype not in _native.DTYPES:
-        raise TypeError(f'raw must be float32, float16 or bfloat16, got {raw.dtype}')
-    if raw.ndim < 1 or raw.shape[-1] < 1:
-        raise ValueError(f'raw must be (..., A) with at least one move, got {tuple(raw.shape)}')
-    if not 0 <= k <= _native.TOP_MAX:
-        raise ValueError(f'k must be in 0 .. {_native.TOP_MAX}, got {k}')
-    _native.require_device(*(t for t in (raw, actions, valid) if t is not None))
-    lead, A = raw.shape[:-1], raw.shape[-1]
-    flat = _native.rows_of(raw, A)
-    if actions is not None:
-        if actions.shape != lead:
-            raise ValueError(f'actions must be {tuple(lead)}, got {tuple(actions.shape)}')
-        if actions.is_floating_point() or actions.is_complex() or actions.dtype == torch.bool:
-            raise TypeError(f'actions must be whole numbers, got {actions.dtype}')
-        actions = actions.long().reshape(-1).contiguous()
-    if valid is not None:
-        if valid.dtype != torch.bool:
-            raise TypeError(f'valid must be bool, got {valid.dtype}')
-        valid = _native.rows_of(valid.expand(raw.shape), A)
-    if torch.is_grad_enabled() and raw.requires_grad:
-        logp, entropy, top, top_logp = _LogProbs.apply(flat, actions, valid, k)
-    else:
-        logp, entropy, top, top_logp, _ = _logprobs(flat.detach(), actions, valid, k, False)
+    logp, entropy, best, best_logp = _native.ops().logprobs(raw, actions, valid, k)
     out = arrdict.arrdict()
     if logp is not None:
-        out['logp'] = logp.view(lead)
-    out['entropy'] = entropy.view(lead)
+        out['logp'] = logp
+    out['entropy'] = entropy
     if k:
-        out['top'], out['top_logp'] = top.view(*lead, k), top_logp.view(*lead, k)
+        out['top'], out['top_logp'] = best, best_logp
     return out
 
 

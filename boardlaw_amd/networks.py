@@ -3,7 +3,6 @@ fully-connected residual blocks, masked log-softmax policy head and tanh value h
 (state_dict keys identical to the reference's: body.N.weight/bias/α, policy.core.*, value.core.*)."""
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
 from . import _native, arrdict, heads
@@ -21,73 +20,6 @@ class ReZeroResidual(nn.Linear):
         return x + getattr(self, 'α') * super().forward(F.relu(x))
 
 
-GATES = {'none': 0, 'full': 1, 'channel': 2, 'row': 3}          # BL_GATE_*
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _norm_args(x, y, alpha, post, gate, kind, pre, eps, h_dtype):
-    """The leading arguments of bl_norm_residual and its gradient: x (R,W); y (R,W), or (R,2W) holding the gate behind the values (kind 'packed')."""
-    R, W = x.shape
-    if kind == 'packed':
-        g, gs, code = y.data_ptr() + W * y.element_size(), y.stride(0), GATES['full']
-    else:
-        g, gs, code = _ptr(gate), gate.stride(0) if kind in ('full', 'row') else 0, GATES[kind]
-    return (x.data_ptr(), _native.DTYPES[x.dtype], x.stride(0), _ptr(y), _native.DTYPES[h_dtype], 0 if y is None else y.stride(0), _ptr(alpha),
-            _ptr(post), g, code, gs, _ptr(pre), eps, R, W)
-
-
-def _norm_residual(x, y, alpha, post, gate, kind, pre, eps, h_dtype, want_stats):
-    R, W = x.shape
-    new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=x.device)
-    out = new(x.dtype, R, W) if y is not None else None
-    h = new(h_dtype, R, W) if pre is not None else None
-    stats = new(torch.float32, R, 2) if want_stats else None
-    if R:
-        with _native.on(x.device):
-            _native.check(_native.lib().bl_norm_residual(*_norm_args(x, y, alpha, post, gate, kind, pre, eps, h_dtype), _ptr(out), _ptr(h), _ptr(stats),
-                                                         _native.stream(x.device)))
-    return out, h, stats
-
-
-class _NormResidual(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, x, y, alpha, post, gate, pre, kind, eps, h_dtype):
-        out, h, stats = _norm_residual(x, y, alpha, post, gate, kind, pre, eps, h_dtype, True)
-        ctx.save_for_backward(x, y, alpha, post, gate, pre, stats)
-        ctx.kind, ctx.eps, ctx.h_dtype = kind, eps, h_dtype
-        ctx.set_materialize_grads(False)
-        return out, h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_out, g_h):
-        x, y, alpha, post, gate, pre, stats = ctx.saved_tensors
-        R, W = x.shape
-        new = lambda like: None if like is None else torch.empty(like.shape, dtype=like.dtype, device=x.device)
-        dx, dy, dalpha, dpost, dgate = (new(t) for t in (x, y, alpha, post, gate))
-        dpre = new(pre) if g_h is not None else None
-        if R == 0:
-            return (dx, dy) + tuple(None if t is None else t.zero_() for t in (dalpha, dpost, dgate, dpre)) + (None,) * 3
-        g_out, g_h = (None if g is None else _native.rows_of(g, W) for g in (g_out, g_h))
-        if ctx.kind == 'packed':
-            dg, dgs = dy.data_ptr() + W * dy.element_size(), dy.stride(0)
-        else:
-            dg, dgs = _ptr(dgate), dgate.stride(0) if ctx.kind in ('full', 'row') else 0
-        L = _native.lib()
-        work = torch.empty(L.bl_norm_residual_workspace(R, W), dtype=torch.uint8, device=x.device)
-        with _native.on(x.device):
-            _native.check(L.bl_norm_residual_grad(
-                *_norm_args(x, y, alpha, post, gate, ctx.kind, pre, ctx.eps, ctx.h_dtype), stats.data_ptr(),
-                _ptr(g_out), 0 if g_out is None else g_out.stride(0), _ptr(g_h), 0 if g_h is None else g_h.stride(0),
-                dx.data_ptr(), _ptr(dy), 0 if dy is None else dy.stride(0), dg, dgs, _ptr(dalpha), _ptr(dpost), _ptr(dpre),
-                work.data_ptr(), _native.stream(x.device)))
-        return dx, dy, dalpha, dpost, dgate, dpre, None, None, None
-
-
 def norm_residual(x, y=None, alpha=None, post=None, gate=None, pre=None, eps=1e-5, dtype=None):
     """The residual stream between two blocks in one pass -- norm behind the block, its gate, the residual scale, norm before the next block:
 
@@ -103,48 +35,7 @@ def norm_residual(x, y=None, alpha=None, post=None, gate=None, pre=None, eps=1e-
         dtype  h's type where y is None (default: x's); else it is y's
 
     -> (x_out, h).  Computed in f32, each result rounded once; differentiable (once) in every tensor.  On the GPU only (bl_norm_residual)."""
-    if x.dtype not in _native.DTYPES:
-        raise TypeError(f'x must be float32, float16 or bfloat16, got {x.dtype}')
-    if x.ndim < 1 or not 1 <= x.shape[-1] <= _native.NORM_MAX:
-        raise ValueError(f'x must be (..., W) with W in 1 .. {_native.NORM_MAX}, got {tuple(x.shape)}')
-    lead, W = x.shape[:-1], x.shape[-1]
-    _native.require_device(*(t for t in (x, y, alpha, post, gate, pre) if t is not None))
-    if y is None:
-        if alpha is not None or post is not None or gate is not None or pre is None:
-            raise ValueError('without y there is only h = pre * x / rms(x): alpha, post and gate must be None and pre given')
-    elif y.shape[:-1] != lead or y.shape[-1] not in (W, 2 * W):
-        raise ValueError(f'y must be {(*lead, W)} or {(*lead, 2 * W)}, got {tuple(y.shape)}')
-    h_dtype = y.dtype if y is not None else (dtype or x.dtype)
-    if h_dtype != x.dtype and not (x.dtype == torch.float32 and h_dtype in _native.DTYPES):
-        raise TypeError(f"y (or dtype) must be of x's type, or float16 / bfloat16 beside float32: got {x.dtype} and {h_dtype}")
-    if y is not None and dtype not in (None, y.dtype):
-        raise TypeError("h is of y's type")
-    for name, t, shape in (('alpha', alpha, ()), ('post', post, (W,)), ('pre', pre, (W,))):
-        if t is not None and (t.shape != shape or t.dtype != torch.float32):
-            raise ValueError(f'{name} must be float32 of shape {shape}, got {t.dtype} {tuple(t.shape)}')
-    if not eps >= 0:
-        raise ValueError(f'eps must not be negative, got {eps}')
-    kind = 'none'
-    if y is not None and y.shape[-1] == 2 * W:
-        kind = 'packed'
-        if gate is not None:
-            raise ValueError('y holds the gates already')
-    elif gate is not None:
-        kind = 'channel' if gate.shape == (W,) else 'full' if gate.shape == x.shape else 'row' if gate.shape == (*lead, 1) else None
-        if kind is None:
-            raise ValueError(f'gate must be {(W,)}, {tuple(x.shape)} or {(*lead, 1)}, got {tuple(gate.shape)}')
-        if gate.dtype != (torch.float32 if kind == 'channel' else h_dtype):
-            raise TypeError(f"a gate per channel is float32, any other of y's type: got {gate.dtype}")
-    flat = lambda t, w: None if t is None else _native.rows_of(t, w)
-    solid = lambda t: None if t is None else t.contiguous()
-    xs, ys = flat(x, W), flat(y, y.shape[-1] if y is not None else 0)
-    gs = solid(gate) if kind == 'channel' else flat(gate, gate.shape[-1]) if gate is not None else None
-    tensors = (xs, ys, alpha, solid(post), gs, solid(pre))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        out, h = _NormResidual.apply(*tensors, kind, eps, h_dtype)
-    else:
-        out, h, _ = _norm_residual(tensors[0], tensors[1], alpha, tensors[3], gs, kind, tensors[5], eps, h_dtype, False)
-    return (x if out is None else out.view(x.shape)), (None if h is None else h.view(x.shape))
+    return _native.ops().norm_residual(x, y, alpha, post, gate, pre, eps, dtype)
 
 
 class GatedResidual(nn.Linear):

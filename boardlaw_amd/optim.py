@@ -1,29 +1,9 @@
 """The learner's optimiser for hidden weights: momentum updates orthogonalised by Newton-Schulz products before they are applied.  The
 reference trains with Adam alone (boardlaw/main.py:153); here `training.run(optimizer='muon')` gives the residual blocks' weights
 to Muon and everything else to Adam."""
-import ctypes
-
 import torch
 
 from . import _native, networks
-
-
-def _orthogonalize(mats, steps, eps):
-    """Matrices of one shape, type and device -> contiguous results."""
-    rows, cols = mats[0].shape
-    dev, count = mats[0].device, len(mats)
-    mats = [m.detach().contiguous() for m in mats]
-    # results in one allocation, each matrix on a 16-byte boundary or better
-    size = rows * cols * mats[0].element_size()
-    pitch = -(-size // 16) * 16 // mats[0].element_size()
-    outs = [o[:rows * cols].view(rows, cols) for o in torch.empty((count, pitch), dtype=mats[0].dtype, device=dev).unbind(0)]
-    L = _native.lib()
-    work = torch.empty(L.bl_orthogonalize_workspace(count, rows, cols), dtype=torch.uint8, device=dev)
-    pointers = ctypes.c_void_p * count
-    with _native.on(dev):
-        _native.check(L.bl_orthogonalize(pointers(*[m.data_ptr() for m in mats]), pointers(*[o.data_ptr() for o in outs]), count,
-                                         _native.DTYPES[mats[0].dtype], rows, cols, steps, eps, work.data_ptr(), _native.stream(dev)))
-    return outs
 
 
 def orthogonalize(matrices, steps=5, eps=1e-7):
@@ -34,35 +14,17 @@ def orthogonalize(matrices, steps=5, eps=1e-7):
 
     -> the same structure, types and shapes; f32 sums and 22-bit operands whatever the type.  Matrices of one shape and type are taken
     through it together.  Not differentiable.  On the GPU only (bl_orthogonalize)."""
-    if not isinstance(steps, int) or steps < 1:
-        raise ValueError(f'steps must be a whole number from 1 on, got {steps!r}')
-    if not eps >= 0:
-        raise ValueError(f'eps must not be negative, got {eps}')
-    if isinstance(matrices, torch.Tensor):
-        if matrices.ndim < 2:
-            raise ValueError(f'a matrix or a batch of them is wanted, got {tuple(matrices.shape)}')
-        flat = matrices.reshape(-1, *matrices.shape[-2:])
-        if flat.numel() == 0:
-            _native.require_device(matrices)
-            return torch.empty_like(matrices)
-        return torch.stack(orthogonalize(list(flat.unbind(0)), steps, eps)).view(matrices.shape)
-    groups, outs = {}, [None] * len(matrices)
-    for i, m in enumerate(matrices):
-        if m.dtype not in _native.DTYPES:
-            raise TypeError(f'matrices must be float32, float16 or bfloat16, got {m.dtype}')
-        if m.ndim != 2:
-            raise ValueError(f'matrices must be two-dimensional, got {tuple(m.shape)}')
-        if max(m.shape) > _native.ORTHO_MAX:
-            raise ValueError(f'sides up to {_native.ORTHO_MAX} are supported, got {tuple(m.shape)}')
-        _native.require_device(m)
-        if m.numel() == 0:
-            outs[i] = torch.empty_like(m)
-        else:
-            groups.setdefault((m.shape, m.dtype, m.device), []).append(i)
-    for members in groups.values():
-        for i, o in zip(members, _orthogonalize([matrices[i] for i in members], steps, eps)):
-            outs[i] = o
-    return outs
+    if not isinstance(matrices, torch.Tensor):
+        return _native.ops().orthogonalize(matrices, steps, eps)
+    if matrices.ndim < 2:
+        raise ValueError(f'a matrix or a batch of them is wanted, got {tuple(matrices.shape)}')
+    if matrices.ndim == 2:
+        return _native.ops().orthogonalize([matrices], steps, eps)[0]
+    flat = matrices.detach().reshape(matrices.shape[:-2].numel(), *matrices.shape[-2:])
+    if flat.shape[0] == 0:
+        _native.require_device(matrices)
+        return torch.empty_like(matrices)
+    return torch.stack(_native.ops().orthogonalize(list(flat.unbind(0)), steps, eps)).view(matrices.shape)
 
 
 class Muon(torch.optim.Optimizer):

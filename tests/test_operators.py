@@ -115,7 +115,9 @@ def test_logprobs(R, A, dtype, masked):
         outs = [out.logp, out.entropy]
         if k:
             gs.append(size * torch.randn((R, k), generator=gen, device='cuda')); outs.append(out.top_logp)
-        d, = torch.autograd.grad(outs, raw, gs)
+        d, = torch.autograd.grad(outs, raw, gs, retain_graph=True)
+        with pytest.raises(RuntimeError, match='differentiable once'):
+            torch.autograd.grad(outs, raw, gs, create_graph=True)
         want, mag = plain_logprobs_grad(w, actions, gs[0], gs[1], gs[2] if k else None)
         assert d.dtype == dtype
         # p is as exact as logp; a sum of k gradients adds k roundings; one to the result's type (in f16 also of the smallest steps)
@@ -632,8 +634,8 @@ def test_refusals():
         optim.orthogonalize([z(3, 4, dtype=torch.float64)])
     with pytest.raises(ValueError):
         optim.orthogonalize([z(1, 16385)])
-    for steps in (0, -1, 2.5):
-        with pytest.raises(ValueError):
+    for steps, error in ((0, ValueError), (-1, ValueError), (1001, ValueError), (2.5, TypeError)):
+        with pytest.raises(error):
             optim.orthogonalize(z(3, 4), steps=steps)
     with pytest.raises(ValueError):
         optim.Muon([torch.nn.Parameter(z(3))])
