@@ -13,7 +13,9 @@
 // wave's load is one contiguous KiB and both operands of P Q^T use the same layout.  The accumulator holds 4 consecutive rows of D per
 // lane, which are 4 consecutive k of D^T as an operand: writing D^T costs nothing, writing D as well goes through LDS once per tile.
 // A and A^2 are symmetric: only the tiles on and above the diagonal are computed.
+#include <type_traits>
 #include "bl_train.h"
+#include "bl_host.h"
 
 #pragma clang fp contract(off)
 
@@ -27,12 +29,12 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float SCALE = 8192.f, UNSCALE = 1.f / 8192.f;
-constexpr int TILE = 64, MANY = 32, PARTS = 32;
+constexpr int PAD = 128, MANY = 32, PARTS = 64;
 constexpr int FRAG = 512;                   // halves of one fragment, hi or lo
 
 struct Mats { const void* in[MANY]; void* out[MANY]; };
 
-int up(int v) { return (v + TILE - 1) / TILE * TILE; }
+int up(int v) { return v <= 64 ? 64 : (v + PAD - 1) / PAD * PAD; }        // whole tiles of 64, or of 128
 
 // halves from one fragment pair to the next are 2 FRAG; (rb, kb): 32 rows, 16 k
 __device__ __forceinline__ long frag_at(int rb, int kb, int KB) { return ((long)rb * KB + kb) * (2 * FRAG); }
@@ -43,9 +45,18 @@ __device__ __forceinline__ void split(float v, f16& hi, f16& lo) { hi = (f16)v; 
 template <typename T> __global__ void __launch_bounds__(256) norm_parts_kernel(Mats q, long total, double* parts) {
     __shared__ double lds[4];
     const T* g = (const T*)q.in[blockIdx.y];
-    const long i0 = total * blockIdx.x / PARTS, i1 = total * (blockIdx.x + 1) / PARTS;
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+    const long nv = wide ? total / V : 0, i0 = nv * blockIdx.x / PARTS, i1 = nv * (blockIdx.x + 1) / PARTS;
     double s = 0.;
-    for (long i = i0 + threadIdx.x; i < i1; i += 256) { const double v = (double)(float)g[i]; s += v * v; }
+    for (long i = i0 + threadIdx.x; i < i1; i += 256) {
+        float v[V];
+        load<T, V>(g + i * V, v);
+#pragma unroll
+        for (int k = 0; k < V; k++) s += (double)v[k] * (double)v[k];
+    }
+    const long rest = total - nv * V, j0 = nv * V + rest * blockIdx.x / PARTS, j1 = nv * V + rest * (blockIdx.x + 1) / PARTS;
+    for (long i = j0 + threadIdx.x; i < j1; i += 256) { const double v = (double)(float)g[i]; s += v * v; }
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -57,8 +68,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) lay_out_kernel(Mats q, int m, int n, int tall, float eps, const double* parts, f16* X, f16* XT, long sx) {
     __shared__ float t[32][33];
     const T* g = (const T*)q.in[blockIdx.z];
-    double ss = 0.;
-    for (int p = 0; p < PARTS; p++) ss += parts[blockIdx.z * PARTS + p];
+    double ss = parts[blockIdx.z * PARTS + (threadIdx.x & 63)];
+    for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
     const double inv = (double)SCALE / (sqrt(ss) + (double)eps);
     const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
     for (int e = threadIdx.x; e < 1024; e += 256) {
@@ -92,64 +103,73 @@ struct Product {
     int m, n, tall, dtype;                          // LAST
     int count;
 };
-template <int MODE>
-__global__ void __launch_bounds__(256) product_kernel(Product p, Mats q) {
-    __shared__ uint32_t turn[4][32][33];
-    const int tn = p.N / TILE, tm = p.M / TILE, per = (MODE == GRAM || MODE == POLY) ? tm * (tm + 1) / 2 : tm * tn;
-    const int z = blockIdx.x / per;
-    int t = blockIdx.x - z * per, I, J;
-    if constexpr (MODE == GRAM || MODE == POLY) { J = 0; while ((J + 1) * (J + 2) / 2 <= t) J++; I = t - J * (J + 1) / 2; }
-    else { I = t / tn; J = t - I * tn; }
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int rb = 2 * I + (wave >> 1), cb = 2 * J + (wave & 1), KB = p.K / 16;
-    const f16* P = p.P + z * p.sp + frag_at(rb, 0, KB) + lane * 8;
-    const f16* Q = p.Q + z * p.sq + frag_at(cb, 0, KB) + lane * 8;
-    float16v acc = {};
-#pragma unroll 4
-    for (int kb = 0; kb < KB; kb++) {
-        const half8 ph = *(const half8*)(P + (long)kb * 2 * FRAG), pl = *(const half8*)(P + (long)kb * 2 * FRAG + FRAG);
-        const half8 qh = *(const half8*)(Q + (long)kb * 2 * FRAG), ql = *(const half8*)(Q + (long)kb * 2 * FRAG + FRAG);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+// The summand of a wave's 32 x 32 of D, at fragment row rb and fragment column cb.  A lane holds column c = lane % 32 of D, rows
+// 8 g + 4 (lane / 32) + 0..3: as an operand (D^T), row c and 4 consecutive k
+struct Summand { half4 hi[4], lo[4]; };
+__device__ __forceinline__ long place(int rb, int cb, int g, int MB) {
+    const int lane = threadIdx.x & 63;
+    return frag_at(cb, 2 * rb + (g >> 1), MB) + ((lane & 31) + 32 * (g & 1)) * 8 + 4 * (lane >> 5);
+}
+__device__ __forceinline__ void fetch_summand(Summand& s, const f16* S, int rb, int cb, int MB) {
+#pragma unroll
+    for (int g = 0; g < 4; g++) { const f16* at = S + place(rb, cb, g, MB); s.hi[g] = *(const half4*)at; s.lo[g] = *(const half4*)(at + FRAG); }
+}
+
+template <typename T> __device__ __forceinline__ void store_tall(T* out, const float (&v)[16], int r0, int col, int n, int m) {
+#pragma unroll
+    for (int g = 0; g < 16; g++) { const int r = r0 + 8 * (g >> 2) + (g & 3); if (r < n && col < m) out[(long)r * m + col] = (T)(v[g] * UNSCALE); }
+}
+template <typename T> __device__ __forceinline__ void store_wide(T* out, const float (*t)[33], int r0, int c0, int n, int m) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {              // two rows of the result at a time, 32 consecutive entries of each
+        const int c = c0 + 2 * i + (lane >> 5), r = r0 + (lane & 31);
+        if (r < n && c < m) out[(long)c * n + r] = (T)(t[2 * i + (lane >> 5)][lane & 31] * UNSCALE);
     }
-    // lane: column c = lane % 32 of D, rows 8 g + 4 (lane / 32) + 0..3.  As an operand (D^T): row c, 4 consecutive k
-    const int c = lane & 31, h = lane >> 5, MB = p.M / 16;
+}
+// a wave's 32 x 32 of D, which is n x m, as the result: as it is where the input was tall, else transposed, through LDS
+__device__ __forceinline__ void store_result(const Product& p, void* out, const float (&v)[16], int rb, int cb, uint32_t (*turn)[33]) {
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    if (p.tall) {
+        if (p.dtype == BL_F32) store_tall((float*)out, v, 32 * rb + 4 * h, 32 * cb + c, p.n, p.m);
+        else if (p.dtype == BL_F16) store_tall((f16*)out, v, 32 * rb + 4 * h, 32 * cb + c, p.n, p.m);
+        else store_tall((bf16*)out, v, 32 * rb + 4 * h, 32 * cb + c, p.n, p.m);
+        return;
+    }
+    float (*t)[33] = (float (*)[33])turn;
+#pragma unroll
+    for (int g = 0; g < 16; g++) t[c][8 * (g >> 2) + 4 * h + (g & 3)] = v[g];
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); __builtin_amdgcn_wave_barrier();
+    if (p.dtype == BL_F32) store_wide((float*)out, t, 32 * rb, 32 * cb, p.n, p.m);
+    else if (p.dtype == BL_F16) store_wide((f16*)out, t, 32 * rb, 32 * cb, p.n, p.m);
+    else store_wide((bf16*)out, t, 32 * rb, 32 * cb, p.n, p.m);
+}
+
+// mirror: D is wanted as an operand too
+template <int MODE>
+__device__ __forceinline__ void epilogue(const Product& p, const Mats& q, const float16v& acc, const Summand& sum, int z, int rb, int cb, bool mirror, uint32_t (*turn)[33]) {
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, MB = p.M / 16;
     float v[16];
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-        const long at = frag_at(cb, 2 * rb + (g >> 1), MB) + (c + 32 * (g & 1)) * 8 + 4 * h;
-        half4 sh = {}, sl = {};
-        if (p.S) { sh = *(const half4*)(p.S + z * p.ss + at); sl = *(const half4*)(p.S + z * p.ss + at + FRAG); }
+        const long at = place(rb, cb, g, MB);
         half4 hi, lo;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float s = (float)sh[i] + (float)sl[i];
-            const float d = fmaf(p.gamma, acc[4 * g + i], p.beta * s);
+            const float d = MODE == GRAM ? p.gamma * acc[4 * g + i] : fmaf(p.gamma, acc[4 * g + i], p.beta * ((float)sum.hi[g][i] + (float)sum.lo[g][i]));
             f16 a, b; split(d, a, b); hi[i] = a; lo[i] = b;
             v[4 * g + i] = d;
         }
         if constexpr (MODE != LAST) { *(half4*)(p.D + z * p.sd + at) = hi; *(half4*)(p.D + z * p.sd + at + FRAG) = lo; }
     }
     if constexpr (MODE == LAST) {
-        // D is n x m
-#pragma unroll
-        for (int g = 0; g < 16; g++) {
-            const int r = 32 * rb + 8 * (g >> 2) + 4 * h + (g & 3), col = 32 * cb + c;
-            if (r < p.n && col < p.m) {
-                const long at = p.tall ? (long)r * p.m + col : (long)col * p.n + r;
-                const float d = v[g] * UNSCALE;
-                if (p.dtype == BL_F32) ((float*)q.out[z])[at] = d;
-                else if (p.dtype == BL_F16) ((f16*)q.out[z])[at] = (f16)d;
-                else ((bf16*)q.out[z])[at] = (bf16)d;
-            }
-        }
-    } else if (MODE == NEXT || I != J) {
-        // D itself as an operand: through LDS, a wave's 32 x 32 its own
+        store_result(p, q.out[z], v, rb, cb, turn);
+    } else if (mirror) {
+        // D itself as an operand: through LDS, a wave's 32 x 32 its own (its DS operations go in order)
 #pragma unroll
         for (int g = 0; g < 16; g++) {
             f16 a, b; split(v[g], a, b);
-            turn[wave][8 * (g >> 2) + 4 * h + (g & 3)][c] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
+            turn[8 * (g >> 2) + 4 * h + (g & 3)][c] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); __builtin_amdgcn_wave_barrier();
         const int NB = p.N / 16;
@@ -158,7 +178,7 @@ __global__ void __launch_bounds__(256) product_kernel(Product p, Mats q) {
             half8 hi, lo;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const uint32_t w = turn[wave][c][16 * s + 8 * h + i];
+                const uint32_t w = turn[c][16 * s + 8 * h + i];
                 hi[i] = __builtin_bit_cast(f16, (uint16_t)w); lo[i] = __builtin_bit_cast(f16, (uint16_t)(w >> 16));
             }
             f16* to = p.DT + z * p.sdt + frag_at(rb, 2 * cb + s, NB) + lane * 8;
@@ -168,16 +188,353 @@ __global__ void __launch_bounds__(256) product_kernel(Product p, Mats q) {
     }
 }
 
+// Which tile of which matrix a workgroup has.  Consecutive workgroups go to the 8 XCDs in turn: each of them gets consecutive tiles, whose
+// operands its L2 then holds
+struct Tile { int z, I, J; };
+template <bool SYM, int ROWS, int COLS> __host__ __device__ __forceinline__ int tiles_in(int M, int N) {
+    const int tm = M / ROWS, tn = N / COLS;
+    if constexpr (!SYM) return tm * tn;
+    else if constexpr (ROWS == COLS) return tn * (tn + 1) / 2;
+    else { static_assert(ROWS == 2 * COLS, "two columns of tiles to a row of them"); return tm * (tm + 1); }
+}
+template <bool SYM, int ROWS, int COLS> __device__ __forceinline__ Tile tile_of(const Product& p) {
+    const int per = tiles_in<SYM, ROWS, COLS>(p.M, p.N);
+    const int total = per * p.count, share = total / 8, extra = total % 8, xcd = blockIdx.x % 8;
+    const int id = xcd * share + (xcd < extra ? xcd : extra) + blockIdx.x / 8;
+    Tile t;
+    t.z = id / per;
+    const int i = id - t.z * per;
+    if constexpr (SYM) {                        // the tiles on and above the diagonal, (double) column by column
+        constexpr int F = ROWS / COLS;          // column j of F columns has j + 1 tiles in each
+        int j = (int)((sqrtf(8.f * (i / F) + 1.f) - 1.f) * .5f);
+        while (F * j * (j + 1) / 2 > i) j--;
+        while (F * (j + 1) * (j + 2) / 2 <= i) j++;
+        const int in = i - F * j * (j + 1) / 2;
+        t.J = F * j + in / (j + 1); t.I = in % (j + 1);
+    } else { const int tn = p.N / COLS; t.I = i / tn; t.J = i - t.I * tn; }
+    return t;
+}
+
+// 16 k of 32 F rows of P and 64 rows of Q
+template <int F> struct Frags { half8 ph[F], pl[F], qh[2], ql[2]; };
+template <int F> __device__ __forceinline__ void multiply_add(const Frags<F>& f, float16v (&acc)[F][2]) {
+#pragma unroll
+    for (int i = 0; i < F; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[i], f.qh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < F; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.ql[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < F; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.qh[j], acc[i][j], 0, 0, 0);
+}
+
+// Few tiles: a workgroup of four waves computes 64 x 64 of D, every wave all of it over a quarter of K, straight from memory into
+// registers; the quarters are added through LDS in a fixed order.  A wave multiplies 12 times per 8 KiB it loads and waits for nobody.
+template <int MODE>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 2))) product_64_kernel(Product p, Mats q) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    constexpr int D = 4;                                    // blocks of 16 k on their way
+    const Tile t = tile_of<SYM, 64, 64>(p);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, KB = p.K / 16, n = KB / 4;
+    const int rb = 2 * t.I + (wave >> 1), cb = 2 * t.J + (wave & 1);        // this wave's 32 x 32 in the end
+    Summand sum;
+    if constexpr (MODE != GRAM) fetch_summand(sum, p.S + t.z * p.ss, rb, cb, p.M / 16);
+    // a row of fragments is contiguous; what is asked for beyond it is not loaded and reads as zero
+    const int bytes = KB * 4 * FRAG;
+    const f16* P = p.P + t.z * p.sp + frag_at(2 * t.I, 0, KB);
+    const f16* Q = p.Q + t.z * p.sq + frag_at(2 * t.J, 0, KB);
+    __amdgpu_buffer_rsrc_t rows[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        rows[i] = __builtin_amdgcn_make_buffer_rsrc((void*)((i < 2 ? P : Q) + (i & 1) * frag_at(1, 0, KB)), 0, bytes, 0x00020000);
+    auto fetch = [&](Frags<2>& f, int kb) {                    // kb of this wave's n
+        const int at = kb < n ? ((wave * n + kb) * 4 * FRAG + lane * 16) : bytes;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            f.ph[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rows[i], at, 0, 0));
+            f.pl[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rows[i], at + 2 * FRAG, 0, 0));
+            f.qh[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rows[2 + i], at, 0, 0));
+            f.ql[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rows[2 + i], at + 2 * FRAG, 0, 0));
+        }
+    };
+    Frags<2> f[D];
+#pragma unroll
+    for (int d = 0; d < D; d++) fetch(f[d], d);
+    float16v acc[2][2] = {};
+    for (int k = 0; k < n; k += D) {
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            multiply_add(f[d], acc);
+            fetch(f[d], k + d + D);
+        }
+    }
+    // lds[tile][wave][value][lane]: every wave leaves the three tiles that are not its own
+    float* lds = (float*)smem;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i != wave)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4)
+                *(float4*)(lds + ((i * 4 + wave) * 4 + v / 4) * 256 + lane * 4) = make_float4(acc[i >> 1][i & 1][v], acc[i >> 1][i & 1][v + 1], acc[i >> 1][i & 1][v + 2], acc[i >> 1][i & 1][v + 3]);
+    __syncthreads();
+    float16v own = wave == 0 ? acc[0][0] : wave == 1 ? acc[0][1] : wave == 2 ? acc[1][0] : acc[1][1], total = {};
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+            float4 o = make_float4(own[v], own[v + 1], own[v + 2], own[v + 3]);
+            if (w != wave) o = *(const float4*)(lds + ((wave * 4 + w) * 4 + v / 4) * 256 + lane * 4);
+            total[v] += o.x; total[v + 1] += o.y; total[v + 2] += o.z; total[v + 3] += o.w;
+        }
+    __syncthreads();
+    epilogue<MODE>(p, q, total, sum, t.z, rb, cb, !SYM || t.I != t.J, (uint32_t (*)[33])(smem + wave * 32 * 33 * 4));
+}
+
+// Many tiles: a workgroup of four waves computes 64 F x 128 of D, each wave 32 F x 64.  16 k at a time go through LDS, which holds four such
+// stages: while stage s is multiplied, the fragments of stage s + 1 are read, stage s + 3 is written from registers and stage s + 7
+// sets out for them -- one barrier per stage, nothing to wait for behind it, and four stages of products for a load to arrive.
+// Stages beyond the last are loaded from the last again and never used, so that a stage is one straight run of instructions, dealt
+// out between the products by the scheduling groups.  F = 4 takes 72 KiB of LDS traffic to 768 cycles of products (F = 2: 48 to 384, which is
+// all that LDS has).
+template <int MODE, int F>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) product_wide_kernel(Product p, Mats q) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    constexpr int NL = F + 2, STAGE = NL * 2048;            // 16-byte loads of a thread per stage; halves
+    f16* lds = (f16*)smem;
+    const Tile t = tile_of<SYM, 64 * F, 128>(p);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 1, wn = wave & 1;
+    const int KB = p.K / 16;
+    // load i: rows of fragments 2 i and 2 i + 1, half of the workgroup each
+    const long mine = frag_at(threadIdx.x >> 7, 0, KB) + (threadIdx.x & 127) * 8;
+    const f16* P = p.P + t.z * p.sp + frag_at(2 * F * t.I, 0, KB) + mine;
+    const f16* Q = p.Q + t.z * p.sq + frag_at(4 * t.J, 0, KB) + mine;
+    half8 r[4][NL];
+    auto fetch = [&](half8 (&r)[NL], int s) {
+        const long at = (long)(s < KB ? s : KB - 1) * 2 * FRAG;
+#pragma unroll
+        for (int i = 0; i < NL; i++) r[i] = *(const half8*)((i < F ? P + frag_at(2 * i, 0, KB) : Q + frag_at(2 * (i - F), 0, KB)) + at);
+    };
+    auto put = [&](const half8 (&r)[NL], int slot) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) *(half8*)(lds + slot * STAGE + i * 2048 + threadIdx.x * 8) = r[i];
+    };
+    auto read = [&](Frags<F>& f, int slot) {
+        const f16* ps = lds + slot * STAGE + F * wm * 2 * FRAG + lane * 8;
+        const f16* qs = lds + slot * STAGE + (2 * F + 2 * wn) * 2 * FRAG + lane * 8;
+#pragma unroll
+        for (int i = 0; i < F; i++) { f.ph[i] = *(const half8*)(ps + i * 2 * FRAG); f.pl[i] = *(const half8*)(ps + i * 2 * FRAG + FRAG); }
+#pragma unroll
+        for (int i = 0; i < 2; i++) { f.qh[i] = *(const half8*)(qs + i * 2 * FRAG); f.ql[i] = *(const half8*)(qs + i * 2 * FRAG + FRAG); }
+    };
+#pragma unroll
+    for (int s = 0; s < 4; s++) fetch(r[s], s);
+#pragma unroll
+    for (int s = 0; s < 3; s++) { put(r[s], s); fetch(r[s], s + 4); }
+    float16v acc[F][2] = {};
+    Frags<F> f[2];
+    __syncthreads();
+    read(f[0], 0);
+    auto stage = [&](auto slot_, int s) {                   // stage s, in slot s % 4
+        constexpr int slot = decltype(slot_)::value, next = (slot + 1) % 4, free = (slot + 3) % 4;
+        __builtin_amdgcn_sched_barrier(0);
+        read(f[(slot + 1) & 1], next);
+        put(r[free], free);
+        fetch(r[free], s + 7);
+        multiply_add<F>(f[slot & 1], acc);
+#pragma unroll
+        for (int i = 0; i < 2 * NL; i++) {                  // reads first, writes and loads in turn behind them, products throughout
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (i & 1) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, F == 4 ? 1 : 0, 0);
+            if (i & 1) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 6 * F, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
+    };
+    for (int s = 0; s < KB; s += 4) {                       // (K is a multiple of 128)
+        stage(std::integral_constant<int, 0>(), s);
+        stage(std::integral_constant<int, 1>(), s + 1);
+        stage(std::integral_constant<int, 2>(), s + 2);
+        stage(std::integral_constant<int, 3>(), s + 3);
+    }
+#pragma unroll
+    for (int i = 0; i < F; i++) {
+        const int rb = 2 * F * t.I + F * wm + i;
+        Summand sum[2];
+        if constexpr (MODE != GRAM) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) fetch_summand(sum[j], p.S + t.z * p.ss, rb, 4 * t.J + 2 * wn + j, p.M / 16);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int cb = 4 * t.J + 2 * wn + j;
+            // D^T of this 32 x 32 is stored in any case; D unless the tile that holds (cb, rb) is computed and stores it
+            const bool mirror = !SYM || rb / 4 < (cb / (2 * F)) * (F / 2);
+            epilogue<MODE>(p, q, acc[i][j], sum[j], t.z, rb, cb, mirror, (uint32_t (*)[33])(smem + wave * 32 * 33 * 4));
+        }
+    }
+}
+
+// ---- m <= 64 and n <= 64 NB: one workgroup takes a matrix through all of it in LDS ------------------------------------------------------
+// 15 dependent products of a few hundred cycles each: launches (3 to 5 us apiece) would be nearly all of the time.
+template <typename T, int NB>
+__global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int steps, float eps) {
+    extern __shared__ __align__(16) char smem[];
+    __shared__ double sums[4];
+    constexpr int NP = 64 * NB, EACH = 64 * NP / 256;
+    f16 *X = (f16*)smem, *XT = X + 2 * 64 * NP, *A = XT + 2 * 64 * NP, *B = A + 2 * 64 * 64;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, m = p.m, n = p.n;
+    const T* g = (const T*)q.in[blockIdx.x];
+    // element (row, k) of an operand with KB blocks of 16 k
+    auto at = [](int row, int k, int KB) { return (int)frag_at(row >> 5, k >> 4, KB) + ((row & 31) + 32 * ((k >> 3) & 1)) * 8 + (k & 7); };
+    auto set = [&](f16* to, int i, float v) { f16 a, b; split(v, a, b); to[i] = a; to[i + FRAG] = b; };
+    float v[EACH];
+    double ss = 0.;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const int e = threadIdx.x + 256 * i, r = p.tall ? e % 64 : e / NP, col = p.tall ? e / 64 : e % NP;
+        const bool in = r < m && col < n;
+        const float x = (float)g[in ? (p.tall ? col * m + r : r * n + col) : 0];
+        v[i] = in ? x : 0.f;
+        ss += (double)v[i] * (double)v[i];
+    }
+    for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
+    if (lane == 0) sums[wave] = ss;
+    __syncthreads();
+    const double inv = (double)SCALE / (sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + (double)eps);
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const int e = threadIdx.x + 256 * i, r = p.tall ? e % 64 : e / NP, col = p.tall ? e / 64 : e % NP;
+        const float x = (float)((double)v[i] * inv);
+        set(X, at(r, col, NP / 16), x);
+        set(XT, at(col, r, 4), x);
+    }
+    __syncthreads();
+    // 32 x 32 of P Q^T at fragment row rb and column cb
+    auto product = [&](const f16* P, const f16* Q, int rb, int cb, int KB) {
+        float16v acc = {};
+#pragma unroll 4
+        for (int kb = 0; kb < KB; kb++) {
+            const f16 *a = P + frag_at(rb, kb, KB) + lane * 8, *b = Q + frag_at(cb, kb, KB) + lane * 8;
+            const half8 ph = *(const half8*)a, pl = *(const half8*)(a + FRAG), qh = *(const half8*)b, ql = *(const half8*)(b + FRAG);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+        }
+        return acc;
+    };
+    // beta S + gamma acc into D^T (laid out like S), its values kept
+    auto finish = [&](float16v& acc, const f16* S, f16* D, int rb, int cb, int MB, float beta, float gamma) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const long to = place(rb, cb, k, MB);
+            half4 hi = {}, lo = {};
+            if (S) { hi = *(const half4*)(S + to); lo = *(const half4*)(S + to + FRAG); }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                acc[4 * k + i] = fmaf(gamma, acc[4 * k + i], beta * ((float)hi[i] + (float)lo[i]));
+                f16 a, b; split(acc[4 * k + i], a, b); hi[i] = a; lo[i] = b;
+            }
+            *(half4*)(D + to) = hi; *(half4*)(D + to + FRAG) = lo;
+        }
+    };
+    const int rb = wave >> 1, cb = wave & 1;
+    for (int it = 0; it < steps; it++) {
+        float16v acc = product(X, X, rb, cb, NP / 16);
+        finish(acc, nullptr, A, rb, cb, 4, 0.f, UNSCALE);
+        __syncthreads();
+        acc = product(A, A, rb, cb, 4);
+        finish(acc, A, B, rb, cb, 4, NS_B, NS_C * UNSCALE);
+        __syncthreads();
+        // X^T B, NP x 64: blocks rb + 2 j of its rows; X is each lane's own to replace, X^T only when every wave has read it
+        float16v next[NB];
+#pragma unroll
+        for (int j = 0; j < NB; j++) { next[j] = product(XT, B, rb + 2 * j, cb, 4); finish(next[j], X, X, rb + 2 * j, cb, NP / 16, NS_A, UNSCALE); }
+        __syncthreads();
+        if (it + 1 == steps) {                  // (A and B are free: the way to the result)
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                float o[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[i] = next[j][i];
+                store_result(p, q.out[blockIdx.x], o, rb + 2 * j, cb, (uint32_t (*)[33])((char*)A + wave * 32 * 33 * 4));
+            }
+            break;
+        }
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) set(XT, at(32 * (rb + 2 * j) + 8 * (i >> 2) + 4 * h + (i & 3), 32 * cb + c, 4), next[j][i]);
+        __syncthreads();
+    }
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------------------------
 struct Plan { long x, a, norm; long total(int count) const { return count * (3 * x + 2 * a) * (long)sizeof(f16) + norm; } };
 Plan plan_of(int m, int n) {                // halves of one matrix: X (and each X^T), A (and B); bytes of the norms' parts
     const long mp = up(m), np = up(n);
     return {2 * mp * np, 2 * mp * mp, MANY * PARTS * (long)sizeof(double)};
 }
-template <int MODE> void multiply(const Product& p, const Mats& q, hipStream_t s) {
-    const int tm = p.M / TILE, tn = p.N / TILE;
-    const long per = (MODE == GRAM || MODE == POLY) ? (long)tm * (tm + 1) / 2 : (long)tm * tn;
-    hipLaunchKernelGGL((product_kernel<MODE>), dim3((unsigned)(per * p.count)), dim3(256), 0, s, p, q);
+template <int MODE, int F> bool wide(const Product& p, const Mats& q, hipStream_t s) {
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    constexpr size_t bytes = 4 * (F + 2) * 4096;
+    static size_t raised[64];
+    if (!bl_raise_lds_limit((const void*)product_wide_kernel<MODE, F>, bytes, raised)) return false;
+    hipLaunchKernelGGL((product_wide_kernel<MODE, F>), dim3((unsigned)(tiles_in<SYM, 64 * F, 128>(p.M, p.N) * p.count)), dim3(256), bytes, s, p, q);
+    return true;
+}
+template <int MODE> bool multiply(const Product& p, const Mats& q, hipStream_t s) {
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    // The larger tile wherever it fills the chip well enough.  us for all 15 products of 5 steps on tiles of 64 x 64 / 128 x 128 / 256 x 128:
+    // 8 matrices of 512: 220 / 256 / 389; of 1024, one: 206 / 338 / 557, two: 309 / 364 / 572, four: 502 / 443 / 596, eight: 845 / 840 / 757; one of 2048:
+    // 942 / 753 / 1010.  In tiles of these products: 256 x 128 pays from 160 of them on (72 .. 128 do not), 128 x 128 from 136 (72 .. 128 do not).
+    if (p.M % 256 == 0 && p.N % 128 == 0 && tiles_in<SYM, 256, 128>(p.M, p.N) * p.count >= 160) return wide<MODE, 4>(p, q, s);
+    if (p.M % 128 == 0 && p.N % 128 == 0 && tiles_in<SYM, 128, 128>(p.M, p.N) * p.count > 128) return wide<MODE, 2>(p, q, s);
+    hipLaunchKernelGGL((product_64_kernel<MODE>), dim3((unsigned)(tiles_in<SYM, 64, 64>(p.M, p.N) * p.count)), dim3(256), 65536, s, p, q);
+    return true;
+}
+
+template <typename T, int NB> bool small(const Product& p, const Mats& q, int steps, float eps, hipStream_t s) {
+    constexpr size_t bytes = 2 * sizeof(f16) * (2 * 64 * 64 * NB + 2 * 64 * 64);
+    static size_t raised[64];
+    if (!bl_raise_lds_limit((const void*)ortho_small_kernel<T, NB>, bytes, raised)) return false;
+    hipLaunchKernelGGL((ortho_small_kernel<T, NB>), dim3(p.count), dim3(256), bytes, s, q, p, steps, eps);
+    return true;
+}
+template <typename T> int run(const Mats& q, int c, int m, int n, int tall, int dtype, int steps, float eps, const Plan& plan, void* workspace, hipStream_t s) {
+    const int mp = up(m), np = up(n);
+    if (m <= 64 && n <= 128) {
+        Product p{};
+        p.m = m; p.n = n; p.tall = tall; p.dtype = dtype; p.count = c;
+        if (!(n <= 64 ? small<T, 1>(p, q, steps, eps, s) : small<T, 2>(p, q, steps, eps, s))) return BL_ELAUNCH;
+        return check_launch();
+    }
+    double* parts = (double*)workspace;
+    f16* X = (f16*)((char*)workspace + plan.norm);
+    f16* XT[2] = {X + c * plan.x, X + 2 * c * plan.x};
+    f16* A = X + 3 * c * plan.x;
+    f16* B = A + c * plan.a;
+    hipLaunchKernelGGL((norm_parts_kernel<T>), dim3(PARTS, c), dim3(256), 0, s, q, (long)m * n, parts);
+    hipLaunchKernelGGL((lay_out_kernel<T>), dim3(np / 32, mp / 32, c), dim3(256), 0, s, q, m, n, tall, eps, parts, X, XT[0], plan.x);
+    for (int it = 0; it < steps; it++) {
+        f16 *from = XT[it & 1], *to = XT[(it & 1) ^ 1];
+        // acc carries SCALE^2
+        bool ok = multiply<GRAM>(Product{X, X, plan.x, plan.x, nullptr, 0, A, A, plan.a, plan.a, mp, mp, np, 0.f, UNSCALE, 0, 0, 0, 0, c}, q, s);
+        ok = ok && multiply<POLY>(Product{A, A, plan.a, plan.a, A, plan.a, B, B, plan.a, plan.a, mp, mp, mp, NS_B, NS_C * UNSCALE, 0, 0, 0, 0, c}, q, s);
+        // X^T B: n x m, whose transpose a X + B X is written over X (nobody reads X here but the lane that replaces it)
+        const Product next{from, B, plan.x, plan.a, X, plan.x, X, to, plan.x, plan.x, np, mp, mp, NS_A, UNSCALE, m, n, tall, dtype, c};
+        ok = ok && (it + 1 < steps ? multiply<NEXT>(next, q, s) : multiply<LAST>(next, q, s));
+        if (!ok) return BL_ELAUNCH;
+    }
+    return check_launch();
 }
 
 }  // namespace
@@ -197,39 +554,15 @@ int bl_orthogonalize(const void* const* host_in, void* const* host_out, int coun
     if (rows > BL_ORTHO_MAX || cols > BL_ORTHO_MAX) return BL_ETOOBIG;
     for (int i = 0; i < count; i++) if (!host_in[i] || !host_out[i]) return BL_EINVAL;
     const hipStream_t s = (hipStream_t)stream;
-    const int tall = rows > cols, m = tall ? cols : rows, n = tall ? rows : cols, mp = up(m), np = up(n);
+    const int tall = rows > cols, m = tall ? cols : rows, n = tall ? rows : cols;
     const Plan plan = plan_of(m, n);
     for (int i0 = 0; i0 < count; i0 += MANY) {
         const int c = count - i0 < MANY ? count - i0 : MANY;
         Mats q{};
         for (int i = 0; i < c; i++) { q.in[i] = host_in[i0 + i]; q.out[i] = host_out[i0 + i]; }
-        double* parts = (double*)workspace;
-        f16* X = (f16*)((char*)workspace + plan.norm);
-        f16* XT[2] = {X + c * plan.x, X + 2 * c * plan.x};
-        f16* A = X + 3 * c * plan.x;
-        f16* B = A + c * plan.a;
-        const dim3 ng(PARTS, c), lg(np / 32, mp / 32, c);
-        if (dtype == BL_F32) {
-            hipLaunchKernelGGL((norm_parts_kernel<float>), ng, dim3(256), 0, s, q, (long)m * n, parts);
-            hipLaunchKernelGGL((lay_out_kernel<float>), lg, dim3(256), 0, s, q, m, n, tall, eps, parts, X, XT[0], plan.x);
-        } else if (dtype == BL_F16) {
-            hipLaunchKernelGGL((norm_parts_kernel<f16>), ng, dim3(256), 0, s, q, (long)m * n, parts);
-            hipLaunchKernelGGL((lay_out_kernel<f16>), lg, dim3(256), 0, s, q, m, n, tall, eps, parts, X, XT[0], plan.x);
-        } else {
-            hipLaunchKernelGGL((norm_parts_kernel<bf16>), ng, dim3(256), 0, s, q, (long)m * n, parts);
-            hipLaunchKernelGGL((lay_out_kernel<bf16>), lg, dim3(256), 0, s, q, m, n, tall, eps, parts, X, XT[0], plan.x);
-        }
-        for (int it = 0; it < steps; it++) {
-            f16 *from = XT[it & 1], *to = XT[(it & 1) ^ 1];
-            // acc carries SCALE^2
-            multiply<GRAM>(Product{X, X, plan.x, plan.x, nullptr, 0, A, A, plan.a, plan.a, mp, mp, np, 0.f, UNSCALE, 0, 0, 0, 0, c}, q, s);
-            multiply<POLY>(Product{A, A, plan.a, plan.a, A, plan.a, B, B, plan.a, plan.a, mp, mp, mp, NS_B, NS_C * UNSCALE, 0, 0, 0, 0, c}, q, s);
-            // X^T B: n x m, whose transpose a X + B X is written over X (nobody reads X here but the lane that replaces it)
-            const Product next{from, B, plan.x, plan.a, X, plan.x, X, to, plan.x, plan.x, np, mp, mp, NS_A, UNSCALE, m, n, tall, dtype, c};
-            if (it + 1 < steps) multiply<NEXT>(next, q, s);
-            else multiply<LAST>(next, q, s);
-        }
-        if (const int rc = check_launch()) return rc;
+        const int rc = dtype == BL_F32 ? run<float>(q, c, m, n, tall, dtype, steps, eps, plan, workspace, s)
+                     : dtype == BL_F16 ? run<f16>(q, c, m, n, tall, dtype, steps, eps, plan, workspace, s) : run<bf16>(q, c, m, n, tall, dtype, steps, eps, plan, workspace, s);
+        if (rc) return rc;
     }
     return BL_OK;
 }

@@ -448,6 +448,21 @@ def test_orthogonalize(m, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('count,m,n', [(1, 64, 128), (2, 128, 64), (33, 50, 100), (9, 512, 512), (20, 512, 512), (8, 1024, 1024), (7, 700, 900), (6, 1030, 500), (1, 2048, 2048)])
+def test_orthogonalize_many(count, m, n):
+    """Batches that take each of the products' tilings, against 64 bits on the device; twice the same."""
+    from boardlaw_amd import optim
+    gen = torch.Generator('cuda').manual_seed(m)
+    mats = [torch.randn((m, n), generator=gen, device='cuda') for _ in range(count)]
+    outs = optim.orthogonalize(mats)
+    for g, o in zip(mats, outs):
+        want = plain_ortho(g)
+        assert (o.double() - want).norm() <= ortho_tolerance(torch.float32, want)
+        assert (o.double() - want).abs().max() <= ortho_tolerance(torch.float32, want)
+    assert all(torch.equal(a, b) for a, b in zip(outs, optim.orthogonalize(mats)))
+
+
+@pytest.mark.gpu
 def test_orthogonalize_borders():
     """Zero, rank one, scales from 1e-30 to 1e30, a list of several shapes and types, views, NaN in one matrix only, more matrices than one launch takes,
     nothing."""
