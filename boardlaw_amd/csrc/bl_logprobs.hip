@@ -16,6 +16,7 @@ namespace {
 
 constexpr int SHORT = 1024;                 // rows up to here stay in a wave's registers
 constexpr int SEGMENT = 4096;               // shortest part of a long row that is worth a workgroup of its own
+constexpr long ONE_WAVE = 2048;             // long rows from which on a wave takes one
 
 struct Rows {
     const void* raw; long raw_stride;       // elements
@@ -64,6 +65,29 @@ __device__ __forceinline__ float given_logp(const Stat& s, float xa, long long a
     return xa == -INFINITY && s.logs == s.logs ? -INFINITY : (xa - s.m) - s.logs;
 }
 
+// m: the maximum so far (-inf: nothing yet), c entries equal to it, r and t over the others
+struct Part { float m, c, r, t; };
+// N more entries into a lane's sums, p.m their maximum already.  An entry costs one exponential and eight other instructions: -inf needs no test, because
+// e^-inf = 0 meets a clamped d (the reference is finite unless it is +inf), and NaN comes through both sums
+template <int N> __device__ __forceinline__ void eat(Part& p, const float (&x)[N]) {
+    const float ref = fmaxf(p.m, -3.402823466e38f);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float d = x[i] - ref;
+        const bool is = x[i] == ref;
+        const float e = is ? 0.f : exp_neg(d);
+        c += is; p.r += e; p.t = fmaf(e, fmaxf(d, -3e38f), p.t);
+    }
+    p.c += (float)c;
+}
+template <int N> __device__ __forceinline__ float max_of(const float (&x)[N]) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) m = fmaxf(m, x[i]);
+    return m;
+}
+
 // ---- short rows: G lanes hold a row, N entries each -----------------------------------------------------------------------------
 // Entry j of the row is with lane j % G.  Loads are coalesced whatever the rows' alignment; everything else is in registers, the
 // reductions are DPP.  What bounds it is instructions per row, not bytes, so up to 256 entries four rows share a wave.
@@ -89,20 +113,12 @@ __global__ void __launch_bounds__(256) logprobs_rows_kernel(Rows q) {
 #pragma unroll
     for (int i = 0; i < N; i++) x[i] = gl + G * i < q.A ? x[i] : -INFINITY;
 
-    float m = x[0];
+    Part p = {reduce<G, Max>(max_of(x)), 0.f, 0.f, 0.f};
+    eat(p, x);
+    float xa = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < N; i++) m = fmaxf(m, x[i]);
-    m = reduce<G, Max>(m);
-    float c = 0.f, r = 0.f, t = 0.f, xa = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const bool is = x[i] == m, dead = x[i] == -INFINITY;
-        const float d = x[i] - m, e = (is || dead) ? 0.f : exp_neg(d);
-        c += is ? 1.f : 0.f; r += e; t += (is || dead) ? 0.f : e * (d < -3e38f ? -3e38f : d);
-        xa = (gl + G * i == a) ? x[i] : xa;
-    }
-    c = reduce<G, Sum>(c); r = reduce<G, Sum>(r); t = reduce<G, Sum>(t);
-    const Stat s = finish(m, c, r, t);
+    for (int i = 0; i < N; i++) xa = (gl + G * i == a) ? x[i] : xa;
+    const Stat s = finish(p.m, reduce<G, Sum>(p.c), reduce<G, Sum>(p.r), reduce<G, Sum>(p.t));
     if (q.logp) xa = reduce<G, Max>(xa);
     if (live && gl == 0) {
         if (q.logp) q.logp[row] = given_logp(s, xa, a, q.A);
@@ -192,14 +208,22 @@ __device__ __forceinline__ u64 lane_u64(u64 v, int lane) { return (u64)lane_u((u
 
 // the best `k` <= 64 so far, lane i holding the i-th
 struct Best {
-    u64 mine = 0, least = 0;                // least: the k-th, in every lane
+    u64 mine = 0, least = 0;                // least: the k-th, or a bound under it, in every lane
     __device__ __forceinline__ void insert(u64 cand, int k) {           // cand: the same in every lane
         const int lane = threadIdx.x & 63;
         const int p = __builtin_popcountll(__ballot(mine > cand));
         const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(mine >> 32), 0x138, 0xf, 0xf, false);     // from the lane below
         const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)mine, 0x138, 0xf, 0xf, false);
         mine = lane < p ? mine : (lane == p ? cand : ((u64)hi << 32 | lo));
-        least = lane_u64(mine, k - 1);
+        const u64 kth = lane_u64(mine, k - 1);
+        least = kth > least ? kth : least;
+    }
+    // before the first offers: the k-th largest of the lanes' own maxima bounds the k-th of all from below.  Without it the first entries
+    // to come are inserted and driven out again, k (1 + log(entries / k)) times an insertion's 30 instructions
+    __device__ __forceinline__ void bound(float top, int k) {
+        unsigned u = code(top), best = 0;
+        for (int n = 0; n < k; n++) { best = reduce_max_u<64>(u); u = u == best ? 0u : u; }
+        least = (u64)best << 32;
     }
     __device__ __forceinline__ void offer(u64 own, int k) {             // own: this lane's candidate
         u64 left = __ballot(own > least);
@@ -211,7 +235,6 @@ struct Best {
     }
 };
 
-struct Part { float m, c, r, t; };
 __device__ __forceinline__ void join(Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m);
     const bool ea = a.m == m, eb = b.m == m;
@@ -266,102 +289,100 @@ template <typename T, int VEC> __device__ __forceinline__ Span span_of(const T* 
     s.v0 = (int)((long)nv * part / S); s.v1 = (int)((long)nv * (part + 1) / S);
     return s;
 }
-// VEC entries from `j` on, -inf where invalid
-template <typename T, int VEC> __device__ __forceinline__ void entries(const T* x0, const uint8_t* v0, int j, float (&x)[VEC]) {
-    load<T, VEC>(x0 + j, x);
-    if (v0) {
-        if constexpr (VEC > 1) {
-            if ((reinterpret_cast<uintptr_t>(v0 + j) & (VEC - 1)) == 0) {
-                const vec<uint8_t, VEC> v = *(const vec<uint8_t, VEC>*)(v0 + j);
+// VEC entries from `j` on as they lie in memory, with their mask; and as floats, -inf where invalid.  Two steps, so that the loads of
+// several of them go out before the first is waited for (a mask behind a branch made every load wait for the one before: 161 against
+// 79 us for 4096 x 32000 bf16)
+template <typename T, int VEC, bool MASK> struct Entries {
+    vec<T, VEC> x;
+    vec<uint8_t, VEC> v;
+    __device__ __forceinline__ void fetch(const T* x0, const uint8_t* v0, int j) {
+        x = *(const vec<T, VEC>*)(x0 + j);
+        if constexpr (MASK) v = *(const vec<uint8_t, VEC>*)(v0 + j);
+    }
+    __device__ __forceinline__ void get(float (&o)[VEC], bool in) const {
 #pragma unroll
-                for (int i = 0; i < VEC; i++) x[i] = v[i] ? x[i] : -INFINITY;
-                return;
-            }
+        for (int i = 0; i < VEC; i++) {
+            bool ok = in;
+            if constexpr (MASK) ok = ok && v[i];
+            o[i] = ok ? (float)x[i] : -INFINITY;
         }
-#pragma unroll
-        for (int i = 0; i < VEC; i++) x[i] = v0[j + i] ? x[i] : -INFINITY;
     }
-}
+};
+template <typename T> __device__ __forceinline__ float entry(const T* x0, const uint8_t* v0, int j) { return !v0 || v0[j] ? (float)x0[j] : -INFINITY; }
 
-// N more entries into a lane's running sums: the maximum first, so that every entry needs one exponential
-template <int N> __device__ __forceinline__ void eat(Part& p, const float (&x)[N], float top) {
-    if (top > p.m) {
-        Part q = {top, 0.f, 0.f, 0.f};
-        join(p, q);
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const bool is = x[i] == p.m, dead = x[i] == -INFINITY;
-        const float d = x[i] - p.m, e = (is || dead) ? 0.f : exp_neg(d);
-        p.c += is ? 1.f : 0.f; p.r += e; p.t += (is || dead) ? 0.f : e * (d < -3e38f ? -3e38f : d);
-    }
-}
-template <int N> __device__ __forceinline__ float max_of(const float (&x)[N]) {
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < N; i++) m = fmaxf(m, x[i]);
-    return m;
-}
-
-template <typename T, int VEC>
+// WAVES waves to a part of a row: four, or one where there are rows enough to fill the chip with it -- a wave that sees more of a row
+// inserts fewer alternatives that are driven out again, and nothing is joined
+template <typename T, int VEC, bool MASK, int WAVES>
 __global__ void __launch_bounds__(256) logprobs_long_kernel(Rows q) {
     __shared__ Part parts[4];
     __shared__ u64 lists[4][64];
-    const long row = blockIdx.x / q.S;
-    const int part = (int)(blockIdx.x - row * q.S), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int TH = 64 * WAVES;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % WAVES, tid = threadIdx.x % TH;
+    const long job = (long)blockIdx.x * (4 / WAVES) + threadIdx.x / TH, row = job / q.S;
+    const int part = (int)(job - row * q.S);
+    if (WAVES == 1 && row >= q.R) return;
     const T* x0 = (const T*)q.raw + row * q.raw_stride;
     const uint8_t* v0 = q.valid ? q.valid + row * q.valid_stride : nullptr;
     const Span s = span_of<T, VEC>(x0, q.A, part, q.S);
     Part p = {-INFINITY, 0.f, 0.f, 0.f};
     Best best;
-    constexpr int U = VEC == 1 ? 8 : 4;                      // vectors of a lane in flight
-    for (int v = s.v0 + tid; __any(v < s.v1); v += 256 * U) {
+    constexpr int U = VEC == 1 ? 8 : VEC == 4 ? 4 : 2;       // vectors of a lane in flight: 8 or 16 entries, at 6 to 8 waves per SIMD
+    for (int v = s.v0 + tid; __any(v < s.v1); v += TH * U) {
+        Entries<T, VEC, MASK> raw[U];
         float x[U][VEC];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int at = v + 256 * u;
-            entries<T, VEC>(x0, v0, s.head + VEC * (at < s.v1 ? at : s.v1 - 1), x[u]);
-        }
+        for (int u = 0; u < U; u++) { const int at = v + TH * u; raw[u].fetch(x0, v0, s.head + VEC * (at < s.v1 ? at : s.v1 - 1)); }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-#pragma unroll
-            for (int i = 0; i < VEC; i++) x[u][i] = v + 256 * u < s.v1 ? x[u][i] : -INFINITY;
-        }
+        for (int u = 0; u < U; u++) raw[u].get(x[u], v + TH * u < s.v1);
         float tops[U];
 #pragma unroll
         for (int u = 0; u < U; u++) tops[u] = max_of(x[u]);
         const float top = max_of(tops);
+        if (top > p.m) { const Part higher = {top, 0.f, 0.f, 0.f}; join(p, higher); }
 #pragma unroll
-        for (int u = 0; u < U; u++) eat<VEC>(p, x[u], u == 0 ? top : -INFINITY);
+        for (int u = 0; u < U; u++) eat(p, x[u]);
         if (q.k) {
+            if (v - tid == s.v0) best.bound(top, q.k);
 #pragma unroll
-            for (int u = 0; u < U; u++)
+            for (int u = 0; u < U; u++) {
                 // (a NaN hides from the maximum but not from the sum)
-                if (__any(code(tops[u]) >= (unsigned)(best.least >> 32) || p.r != p.r))
+                u64 hits = __ballot(code(tops[u]) >= (unsigned)(best.least >> 32) || p.r != p.r);
+                if constexpr (VEC == 1) { if (hits) best.offer(pack(x[u][0], v + TH * u), q.k); }
+                else while (hits) {                 // few: one lane's entries, dealt out to lanes 0 .. VEC - 1
+                    const int from = __builtin_ctzll(hits);
+                    hits &= hits - 1;
+                    float mine = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) best.offer(pack(x[u][i], s.head + VEC * (v + 256 * u) + i), q.k);
+                    for (int i = 0; i < VEC; i++) { const float o = lane_f(x[u][i], from); mine = lane == i ? o : mine; }
+                    best.offer(pack(mine, s.head + VEC * (v - lane + from + TH * u) + lane), q.k);
+                }
+            }
         }
     }
-    // the single entries: wave 0 takes the head of the first part, wave 1 the tail of the last
-    const int singles = wave == 0 && part == 0 ? s.head : (wave == 1 && part == q.S - 1 ? q.A - s.tail : 0);
-    if (VEC > 1 && singles > 0) {
-        const int j = (wave == 0 ? 0 : s.tail) + lane;
-        float x[1] = {-INFINITY};
-        if (lane < singles) entries<T, 1>(x0, v0, j, x);
-        eat<1>(p, x, x[0]);
-        if (q.k) best.offer(pack(x[0], j), q.k);
+    // the single entries before the first part's vectors and behind the last's, under 8 each
+    if (VEC > 1 && wave == 0) {
+        const bool front = part == 0 && lane < s.head, back = part == q.S - 1 && lane >= 8 && lane - 8 < q.A - s.tail;
+        if (__any(front || back)) {
+            const int j = front ? lane : s.tail + lane - 8;
+            const float x[1] = {front || back ? entry(x0, v0, j) : -INFINITY};
+            if (x[0] > p.m) { const Part higher = {x[0], 0.f, 0.f, 0.f}; join(p, higher); }
+            eat(p, x);
+            if (q.k) best.offer(pack(x[0], j), q.k);
+        }
     }
     p = wave_join(p);
-    if (lane == 0) parts[wave] = p;
-    lists[wave][lane] = best.mine;
-    __syncthreads();
-    if (wave) return;
-    for (int w = 1; w < 4; w++) {
-        join(p, parts[w]);
-        if (q.k) best.offer(lane < q.k ? lists[w][lane] : 0ull, q.k);
+    if constexpr (WAVES > 1) {
+        if (lane == 0) parts[wave] = p;
+        lists[wave][lane] = best.mine;
+        __syncthreads();
+        if (wave) return;
+        for (int w = 1; w < WAVES; w++) {
+            join(p, parts[w]);
+            if (q.k) best.offer(lane < q.k ? lists[w][lane] : 0ull, q.k);
+        }
     }
     if (q.S == 1) { finish_row<T>(q, row, p, best); return; }
-    char* to = q.parts + ((long)blockIdx.x) * (sizeof(Part) + 8l * q.k);
+    char* to = q.parts + job * (sizeof(Part) + 8l * q.k);
     if (lane == 0) *(Part*)to = p;
     if (lane < q.k) ((u64*)(to + sizeof(Part)))[lane] = best.mine;
 }
@@ -385,7 +406,7 @@ __global__ void __launch_bounds__(64) logprobs_join_kernel(Rows q) {
     finish_row<T>(q, row, p, best);
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool MASK>
 __global__ void __launch_bounds__(256) logprobs_long_grad_kernel(Grads q) {
     const long row = blockIdx.x / q.S;
     const int part = (int)(blockIdx.x - row * q.S), tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -408,20 +429,25 @@ __global__ void __launch_bounds__(256) logprobs_long_grad_kernel(Grads q) {
         const float g = (j == a ? ga : 0.f) - (pr == 0.f ? 0.f : pr * w);
         return x == -INFINITY ? 0.f : g;
     };
-    for (int v = s.v0 + tid; v < s.v1; v += 256) {
-        float x[VEC], o[VEC];
-        const int j = s.head + VEC * v;
-        entries<T, VEC>(x0, v0, j, x);
+    constexpr int U = VEC == 1 ? 8 : 4;
+    for (int v = s.v0 + tid; v < s.v1; v += 256 * U) {
+        Entries<T, VEC, MASK> raw[U];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) o[i] = grad(x[i], j + i);
-        store<T, VEC>(d0 + j, o);
+        for (int u = 0; u < U; u++) { const int at = v + 256 * u; raw[u].fetch(x0, v0, s.head + VEC * (at < s.v1 ? at : s.v1 - 1)); }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = s.head + VEC * (v + 256 * u);
+            float x[VEC], o[VEC];
+            raw[u].get(x, true);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o[i] = grad(x[i], j + i);
+            if (v + 256 * u < s.v1) store<T, VEC>(d0 + j, o);
+        }
     }
     const int singles = wave == 0 && part == 0 ? s.head : (wave == 1 && part == q.S - 1 ? q.A - s.tail : 0);
     if (VEC > 1 && lane < singles) {
         const int j = (wave == 0 ? 0 : s.tail) + lane;
-        float x[1];
-        entries<T, 1>(x0, v0, j, x);
-        d0[j] = (T)grad(x[0], j);
+        d0[j] = (T)grad(entry(x0, v0, j), j);
     }
     if (!q.g_top) return;
     // the alternatives' own terms, over what this workgroup has just written
@@ -429,11 +455,7 @@ __global__ void __launch_bounds__(256) logprobs_long_grad_kernel(Grads q) {
     const int lo = part == 0 ? 0 : s.head + VEC * s.v0, hi = part == q.S - 1 ? q.A : s.head + VEC * s.v1;
     if (tid < q.k) {
         const long long j = q.top[row * q.k + tid];
-        if (j >= lo && j < hi) {
-            float x[1];
-            entries<T, 1>(x0, v0, (int)j, x);
-            d0[j] = (T)(grad(x[0], (int)j) + q.g_top[row * q.k + tid]);
-        }
+        if (j >= lo && j < hi) d0[j] = (T)(grad(entry(x0, v0, (int)j), (int)j) + q.g_top[row * q.k + tid]);
     }
 }
 
@@ -446,10 +468,13 @@ int parts_of(long R, int A) {
     long s = want < most ? want : most;
     return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
 }
-// rows whose 16-byte boundaries fall on the same entries in `raw` and in the contiguous result
-bool vectors(const void* raw, long stride, const void* other, int A, int size) {
+// Rows whose 16-byte boundaries fall on the same entries in `raw` and in the contiguous result, and on whole words of the mask: V entries of
+// each at a time.  Otherwise one by one
+bool vectors(const void* raw, long stride, const void* other, const uint8_t* valid, long valid_stride, int A, int size) {
+    const int V = 16 / size;
     if ((reinterpret_cast<uintptr_t>(raw) & 15) || (reinterpret_cast<uintptr_t>(other) & 15)) return false;
-    return stride == A || ((stride * size) % 16 == 0 && ((long)A * size) % 16 == 0);
+    if (valid && ((reinterpret_cast<uintptr_t>(valid) % V) || (valid_stride - stride) % V)) return false;
+    return stride == A || (stride % V == 0 && A % V == 0);
 }
 
 template <typename T, int G, int N> void go_short(const Rows& q, hipStream_t s) {
@@ -472,8 +497,19 @@ template <typename T> int run(const Rows& q, hipStream_t s) {
     if (q.A <= SHORT) { pick_short<T>(q, s); return check_launch(); }
     constexpr int V = 16 / sizeof(T);
     const dim3 grid((unsigned)(q.R * q.S));
-    if (vectors(q.raw, q.raw_stride, q.raw, q.A, sizeof(T))) hipLaunchKernelGGL((logprobs_long_kernel<T, V>), grid, dim3(256), 0, s, q);
-    else hipLaunchKernelGGL((logprobs_long_kernel<T, 1>), grid, dim3(256), 0, s, q);
+    const bool wide = vectors(q.raw, q.raw_stride, q.raw, q.valid, q.valid_stride, q.A, sizeof(T));
+    if (q.R >= ONE_WAVE) {
+        const dim3 grid4((unsigned)((q.R + 3) / 4));
+        if (wide && !q.valid) hipLaunchKernelGGL((logprobs_long_kernel<T, V, false, 1>), grid4, dim3(256), 0, s, q);
+        else if (wide) hipLaunchKernelGGL((logprobs_long_kernel<T, V, true, 1>), grid4, dim3(256), 0, s, q);
+        else if (!q.valid) hipLaunchKernelGGL((logprobs_long_kernel<T, 1, false, 1>), grid4, dim3(256), 0, s, q);
+        else hipLaunchKernelGGL((logprobs_long_kernel<T, 1, true, 1>), grid4, dim3(256), 0, s, q);
+        return check_launch();
+    }
+    if (wide && !q.valid) hipLaunchKernelGGL((logprobs_long_kernel<T, V, false, 4>), grid, dim3(256), 0, s, q);
+    else if (wide) hipLaunchKernelGGL((logprobs_long_kernel<T, V, true, 4>), grid, dim3(256), 0, s, q);
+    else if (!q.valid) hipLaunchKernelGGL((logprobs_long_kernel<T, 1, false, 4>), grid, dim3(256), 0, s, q);
+    else hipLaunchKernelGGL((logprobs_long_kernel<T, 1, true, 4>), grid, dim3(256), 0, s, q);
     if (q.S > 1) hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)q.R), dim3(64), 0, s, q);
     return check_launch();
 }
@@ -481,8 +517,11 @@ template <typename T> int run(const Grads& q, hipStream_t s) {
     if (q.A <= SHORT) { pick_short<T>(q, s); return check_launch(); }
     constexpr int V = 16 / sizeof(T);
     const dim3 grid((unsigned)(q.R * q.S));
-    if (vectors(q.raw, q.raw_stride, q.d_raw, q.A, sizeof(T))) hipLaunchKernelGGL((logprobs_long_grad_kernel<T, V>), grid, dim3(256), 0, s, q);
-    else hipLaunchKernelGGL((logprobs_long_grad_kernel<T, 1>), grid, dim3(256), 0, s, q);
+    const bool wide = vectors(q.raw, q.raw_stride, q.d_raw, q.valid, q.valid_stride, q.A, sizeof(T));
+    if (wide && !q.valid) hipLaunchKernelGGL((logprobs_long_grad_kernel<T, V, false>), grid, dim3(256), 0, s, q);
+    else if (wide) hipLaunchKernelGGL((logprobs_long_grad_kernel<T, V, true>), grid, dim3(256), 0, s, q);
+    else if (!q.valid) hipLaunchKernelGGL((logprobs_long_grad_kernel<T, 1, false>), grid, dim3(256), 0, s, q);
+    else hipLaunchKernelGGL((logprobs_long_grad_kernel<T, 1, true>), grid, dim3(256), 0, s, q);
     return check_launch();
 }
 

@@ -6,7 +6,7 @@
 //     z  = g_x' + rx (t - xn mean(t xn)),  t = g_h pre;      dx = z;      dpre = sum_rows g_h xn;      dalpha = sum z u
 //     dgate = alpha z post n s (1 - s);    dpost = sum_rows alpha z s n;  dy = ry (dn - n mean(dn n)),  dn = alpha z s post
 // Everything is computed in f32 and rounded once at its store.  The bound is HBM: every element is read once and written once; a row
-// is held in registers by G lanes of 8 elements each, so the two dependent sums of a row cost no second read.  The sums over rows are
+// is held in registers by G lanes of N elements each, so the two dependent sums of a row cost no second read.  The sums over rows are
 // kept per workgroup in registers over all of its rows and added up by a second launch in a fixed order: no atomics, the same bits
 // every time.
 #include "bl_train.h"
@@ -16,8 +16,6 @@
 using namespace bltrain;
 
 namespace {
-
-constexpr int N = 8;                        // elements of a row per lane
 
 struct Norm {
     const void* x; long xs;
@@ -31,25 +29,39 @@ struct Norm {
     void* dx; void* dy; long dys; void* dgate; long dgs; float* parts;
 };
 
-// where lane gl's 8 elements of a row are: VEC == 8 together (16-byte accesses), VEC == 1 every G-th
-template <int G, int VEC> __device__ __forceinline__ int column(int gl, int i) { return VEC == 8 ? 8 * gl + i : gl + G * i; }
+// where lane gl's N elements of a row are: VEC == 8 in eights (16-byte accesses), VEC == 1 every G-th
+template <int G, int VEC> __device__ __forceinline__ int column(int gl, int i) { return VEC == 8 ? 8 * (gl + G * (i / 8)) + i % 8 : gl + G * i; }
 
-template <int G, int VEC, typename T> __device__ __forceinline__ void read(const T* p, int gl, int W, float (&o)[N]) {
-    if constexpr (VEC == 8) {
-        if (8 * gl < W) load<T, 8>(p + 8 * gl, o);
-        else
+// A lane's elements as they lie in memory, and as floats (0 beyond W).  Two steps, so that all of a row's tensors are on their way before the first is
+// waited for; the address is clamped instead of a branch around the load
+template <int G, int VEC, int N, typename T> struct Elements {
+    vec<T, VEC> v[N / VEC];
+    __device__ __forceinline__ void fetch(const T* p, int gl, int W) {
 #pragma unroll
-            for (int i = 0; i < N; i++) o[i] = 0.f;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) { const int j = gl + G * i; o[i] = (float)p[j < W ? j : W - 1]; }
-#pragma unroll
-        for (int i = 0; i < N; i++) o[i] = gl + G * i < W ? o[i] : 0.f;
+        for (int c = 0; c < N / VEC; c++) { const int j = column<G, VEC>(gl, c * VEC); v[c] = *(const vec<T, VEC>*)(p + (j < W ? j : W - VEC)); }
     }
+    __device__ __forceinline__ void get(float (&o)[N], int gl, int W) const {
+#pragma unroll
+        for (int c = 0; c < N / VEC; c++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o[c * VEC + i] = column<G, VEC>(gl, c * VEC) < W ? (float)v[c][i] : 0.f;
+    }
+};
+template <int G, int VEC, typename T, int N> __device__ __forceinline__ void read(const T* p, int gl, int W, float (&o)[N]) {
+    Elements<G, VEC, N, T> e;
+    e.fetch(p, gl, W);
+    e.get(o, gl, W);
 }
-template <int G, int VEC, typename T> __device__ __forceinline__ void write(T* p, int gl, int W, const float (&o)[N]) {
+template <int G, int VEC, typename T, int N> __device__ __forceinline__ void write(T* p, int gl, int W, const float (&o)[N]) {
     if constexpr (VEC == 8) {
-        if (8 * gl < W) store<T, 8>(p + 8 * gl, o);
+#pragma unroll
+        for (int c = 0; c < N; c += 8) {
+            const int j = column<G, 8>(gl, c);
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = o[c + i];
+            if (j < W) store<T, 8>(p + j, v);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) { const int j = gl + G * i; if (j < W) p[j] = (T)o[i]; }
@@ -78,27 +90,37 @@ __device__ __forceinline__ Gate sigmoid(float g) {
     return {s, s == 0.f ? 0.f : e * s * s};
 }
 
-template <typename TX, typename TY, int G, int VEC>
+template <typename TX, typename TY, int G, int N, int VEC>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(Norm q) {
     __shared__ float lds[32];
     constexpr int T = G > 256 ? G : 256, ROWS = T / G;
     const int gl = threadIdx.x & (G - 1);
     int set = 0;
     float post[N], pre[N], gate[N];
-    if (q.post) read<G, VEC>(q.post, gl, q.W, post);
-    if (q.pre) read<G, VEC>(q.pre, gl, q.W, pre);
-    if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
+    constexpr bool KEEP = N == 8;           // gains in registers for all rows; 16 elements per lane leave no room, and a row's are read with it
+    auto gains = [&] {
+        if (q.post) read<G, VEC>(q.post, gl, q.W, post);
+        if (q.pre) read<G, VEC>(q.pre, gl, q.W, pre);
+        if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
+    };
+    if constexpr (KEEP) gains();
     const float alpha = q.alpha ? *q.alpha : 1.f;
     for (long r0 = (long)blockIdx.x * ROWS; r0 < q.R; r0 += (long)gridDim.x * ROWS) {
         const long row = r0 + threadIdx.x / G, at = row < q.R ? row : q.R - 1;      // (G > 64: one row per workgroup, always live)
         const bool live = row < q.R;
+        Elements<G, VEC, N, TX> ex;
+        Elements<G, VEC, N, TY> ey, eg;
+        ex.fetch((const TX*)q.x + at * q.xs, gl, q.W);
+        if (q.y) ey.fetch((const TY*)q.y + at * q.ys, gl, q.W);
+        if (q.kind == BL_GATE_FULL) eg.fetch((const TY*)q.gate + at * q.gs, gl, q.W);
+        if constexpr (!KEEP) gains();
         float x[N];
-        read<G, VEC>((const TX*)q.x + at * q.xs, gl, q.W, x);
+        ex.get(x, gl, q.W);
         float ry = 1.f;
         if (q.y) {
             float y[N];
-            read<G, VEC>((const TY*)q.y + at * q.ys, gl, q.W, y);
-            if (q.kind == BL_GATE_FULL) read<G, VEC>((const TY*)q.gate + at * q.gs, gl, q.W, gate);
+            ey.get(y, gl, q.W);
+            if (q.kind == BL_GATE_FULL) eg.get(gate, gl, q.W);
             if (q.kind == BL_GATE_ROW) {
                 const float g = (float)((const TY*)q.gate)[at * q.gs];
 #pragma unroll
@@ -134,7 +156,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(Norm q) {
     }
 }
 
-template <typename TX, typename TY, int G, int VEC>
+template <typename TX, typename TY, int G, int N, int VEC>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
     __shared__ float lds[32];
     constexpr int T = G > 256 ? G : 256, ROWS = T / G;
@@ -142,9 +164,13 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
     const int gl = threadIdx.x & (G - 1);
     int set = 0;
     float post[N], pre[N], gate[N];
-    if (q.post) read<G, VEC>(q.post, gl, q.W, post);
-    if (q.gh) read<G, VEC>(q.pre, gl, q.W, pre);
-    if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
+    constexpr bool KEEP = N == 8;           // gains in registers for all rows; 16 elements per lane leave no room, and a row's are read with it
+    auto gains = [&] {
+        if (q.post) read<G, VEC>(q.post, gl, q.W, post);
+        if (q.gh) read<G, VEC>(q.pre, gl, q.W, pre);
+        if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
+    };
+    if constexpr (KEEP) gains();
     const float alpha = q.alpha ? *q.alpha : 1.f;
     float spost[N], spre[N], sgate[N], salpha = 0.f;
 #pragma unroll
@@ -153,23 +179,30 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
         const long row = r0 + threadIdx.x / G, at = row < q.R ? row : q.R - 1;
         const bool live = row < q.R;
         const float ry = q.stats[2 * at], rx = q.stats[2 * at + 1];
-        float x[N], z[N], n[N], s[N], ds[N], u[N];
-        read<G, VEC>((const TX*)q.x + at * q.xs, gl, q.W, x);
+        Elements<G, VEC, N, TX> ex, ez;
+        Elements<G, VEC, N, TY> ey, eg, et;
+        ex.fetch((const TX*)q.x + at * q.xs, gl, q.W);
+        if (q.y) ey.fetch((const TY*)q.y + at * q.ys, gl, q.W);
+        if (q.kind == BL_GATE_FULL) eg.fetch((const TY*)q.gate + at * q.gs, gl, q.W);
+        if (q.gx) ez.fetch((const TX*)q.gx + at * q.gxs, gl, q.W);
+        if (q.gh) et.fetch((const TY*)q.gh + at * q.ghs, gl, q.W);
+        if constexpr (!KEEP) gains();
+        float x[N], z[N], n[N], s[N], ds[N], u[N], t[N];
+        ex.get(x, gl, q.W);
         if (q.y) {
-            read<G, VEC>((const TY*)q.y + at * q.ys, gl, q.W, n);
-            if (q.kind == BL_GATE_FULL) read<G, VEC>((const TY*)q.gate + at * q.gs, gl, q.W, gate);
+            ey.get(n, gl, q.W);
+            if (q.kind == BL_GATE_FULL) eg.get(gate, gl, q.W);
             if (q.kind == BL_GATE_ROW) {
                 const float g = (float)((const TY*)q.gate)[at * q.gs];
 #pragma unroll
                 for (int i = 0; i < N; i++) gate[i] = g;
             }
         }
-        float t[N];
-        if (q.gx) read<G, VEC>((const TX*)q.gx + at * q.gxs, gl, q.W, z);
+        if (q.gx) ez.get(z, gl, q.W);
         else
 #pragma unroll
             for (int i = 0; i < N; i++) z[i] = 0.f;
-        if (q.gh) read<G, VEC>((const TY*)q.gh + at * q.ghs, gl, q.W, t);
+        if (q.gh) et.get(t, gl, q.W);
         if (q.y) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
@@ -259,50 +292,57 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
     }
 }
 
-// the workgroups' sums added up: 64 columns by 4 parts of the workgroups, then the 4 parts
+// the workgroups' sums added up: 64 columns by 16 parts of the workgroups, then the 16 parts
 struct Sums { const float* parts; int blocks, W; float* dpost; float* dpre; float* dgate; float* dalpha; };
-__global__ void __launch_bounds__(256) norm_sums_kernel(Sums q) {
-    __shared__ float lds[256];
+__global__ void __launch_bounds__(1024) norm_sums_kernel(Sums q) {
+    __shared__ float lds[1024];
     const int C = 3 * q.W + 1, col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    float* to = col < q.W ? q.dpost : col < 2 * q.W ? q.dpre : col < 3 * q.W ? q.dgate : col < C ? q.dalpha : nullptr;
     float v = 0.f;
-    if (col < C) {
-        const int b0 = (int)((long)q.blocks * part / 4), b1 = (int)((long)q.blocks * (part + 1) / 4);
+    if (to) {
+        const int b0 = (int)((long)q.blocks * part / 16), b1 = (int)((long)q.blocks * (part + 1) / 16);
 #pragma unroll 8
         for (int b = b0; b < b1; b++) v += q.parts[(long)b * C + col];
     }
     lds[threadIdx.x] = v;
     __syncthreads();
-    if (part || col >= C) return;
-    v = (lds[threadIdx.x] + lds[threadIdx.x + 64]) + (lds[threadIdx.x + 128] + lds[threadIdx.x + 192]);
-    float* to = col < q.W ? q.dpost : col < 2 * q.W ? q.dpre : col < 3 * q.W ? q.dgate : q.dalpha;
-    if (to) to[col < 3 * q.W ? col % q.W : 0] = v;
+    if (part || !to) return;
+#pragma unroll
+    for (int p = 1; p < 16; p++) v += lds[threadIdx.x + 64 * p];
+    to[col < 3 * q.W ? col % q.W : 0] = v;
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------
-int lanes_of(int W) { return W <= 16 * N ? 16 : W <= 64 * N ? 64 : W <= 256 * N ? 256 : 1024; }
+// Lanes and elements per lane by width: a row in one wave up to 1024 (no barrier; 4096 x 771 f32 forward + backward 50 us in four waves of 8 elements),
+// a row per 16 lanes up to 128 (four rows to a wave)
+struct Lanes { int G, N; };
+Lanes lanes_of(int W) { return W <= 128 ? Lanes{16, 8} : W <= 512 ? Lanes{64, 8} : W <= 1024 ? Lanes{64, 16} : W <= 2048 ? Lanes{256, 8} : W <= 4096 ? Lanes{512, 8} : Lanes{512, 16}; }
 // workgroups of the backward pass: each leaves 3 W + 1 sums, so no more than keep the chip full
 int blocks_of(long R, int W) {
-    const int G = lanes_of(W), rows = G > 256 ? 1 : 256 / G;
-    const long need = (R + rows - 1) / rows, most = G > 256 ? 512 : 1024;
+    const int G = lanes_of(W).G, rows = G > 256 ? 1 : 256 / G;
+    const long need = (R + rows - 1) / rows, most = 512;
     return (int)(need < most ? need : most);
 }
 bool aligned(const void* p, long stride, int size) { return !p || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * size) % 16 == 0); }
 
-template <typename TX, typename TY, int G, int VEC> int go(const Norm& q, bool grad, hipStream_t s) {
+template <typename TX, typename TY, int G, int N, int VEC> int go(const Norm& q, bool grad, hipStream_t s) {
     constexpr int T = G > 256 ? G : 256, ROWS = T / G;
-    if (grad) hipLaunchKernelGGL((norm_grad_kernel<TX, TY, G, VEC>), dim3((unsigned)blocks_of(q.R, q.W)), dim3(T), 0, s, q);
+    if (grad) hipLaunchKernelGGL((norm_grad_kernel<TX, TY, G, N, VEC>), dim3((unsigned)blocks_of(q.R, q.W)), dim3(T), 0, s, q);
     else {
         const long need = (q.R + ROWS - 1) / ROWS;
-        hipLaunchKernelGGL((norm_kernel<TX, TY, G, VEC>), dim3((unsigned)(need < 2048 ? need : 2048)), dim3(T), 0, s, q);
+        hipLaunchKernelGGL((norm_kernel<TX, TY, G, N, VEC>), dim3((unsigned)(need < 2048 ? need : 2048)), dim3(T), 0, s, q);
     }
     return check_launch();
 }
 template <typename TX, typename TY, int VEC> int by_lanes(const Norm& q, bool grad, hipStream_t s) {
-    switch (lanes_of(q.W)) {
-        case 16: return go<TX, TY, 16, VEC>(q, grad, s);
-        case 64: return go<TX, TY, 64, VEC>(q, grad, s);
-        case 256: return go<TX, TY, 256, VEC>(q, grad, s);
-        default: return go<TX, TY, 1024, VEC>(q, grad, s);
+    const Lanes l = lanes_of(q.W);
+    switch (l.G * l.N) {
+        case 128: return go<TX, TY, 16, 8, VEC>(q, grad, s);
+        case 512: return go<TX, TY, 64, 8, VEC>(q, grad, s);
+        case 1024: return go<TX, TY, 64, 16, VEC>(q, grad, s);
+        case 2048: return go<TX, TY, 256, 8, VEC>(q, grad, s);
+        case 4096: return go<TX, TY, 512, 8, VEC>(q, grad, s);
+        default: return go<TX, TY, 512, 16, VEC>(q, grad, s);
     }
 }
 template <typename TX, typename TY> int by_vec(const Norm& q, bool grad, hipStream_t s) {
@@ -360,7 +400,7 @@ int bl_norm_residual_grad(const void* x, int x_dtype, long x_stride, const void*
     if (const int rc = by_type(q, x_dtype, y_dtype, true, (hipStream_t)stream)) return rc;
     if (!d_alpha && !d_post && !d_pre && !(gate_kind == BL_GATE_CHANNEL && d_gate)) return BL_OK;
     Sums t{q.parts, blocks_of(R, W), W, d_post, d_pre, gate_kind == BL_GATE_CHANNEL ? (float*)d_gate : nullptr, d_alpha};
-    hipLaunchKernelGGL(norm_sums_kernel, dim3((unsigned)((3 * W + 1 + 63) / 64)), dim3(256), 0, (hipStream_t)stream, t);
+    hipLaunchKernelGGL(norm_sums_kernel, dim3((unsigned)((3 * W + 1 + 63) / 64)), dim3(1024), 0, (hipStream_t)stream, t);
     return check_launch();
 }
 
