@@ -121,10 +121,13 @@ template <typename T> __device__ __forceinline__ void store_tall(T* out, const f
 }
 template <typename T> __device__ __forceinline__ void store_wide(T* out, const float (*t)[33], int r0, int c0, int n, int m) {
     const int lane = threadIdx.x & 63;
+    float o[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[i] = t[2 * i + (lane >> 5)][lane & 31];
 #pragma unroll
     for (int i = 0; i < 16; i++) {              // two rows of the result at a time, 32 consecutive entries of each
         const int c = c0 + 2 * i + (lane >> 5), r = r0 + (lane & 31);
-        if (r < n && c < m) out[(long)c * n + r] = (T)(t[2 * i + (lane >> 5)][lane & 31] * UNSCALE);
+        if (r < n && c < m) out[(long)c * n + r] = (T)(o[i] * UNSCALE);
     }
 }
 // a wave's 32 x 32 of D, which is n x m, as the result: as it is where the input was tall, else transposed, through LDS
@@ -238,7 +241,7 @@ template <int MODE>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 2))) product_64_kernel(Product p, Mats q) {
     extern __shared__ __align__(16) char smem[];
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
-    constexpr int D = 4;                                    // blocks of 16 k on their way
+    constexpr int D = 2;                                    // blocks of 16 k on their way (1, 2, 3, 4: 4 x 128 x 128 86, 88, 95, 101 us for 5 steps, 4 x 512 x 512 155, 153, 159, 158)
     const Tile t = tile_of<SYM, 64, 64>(p);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, KB = p.K / 16, n = KB / 4;
     const int rb = 2 * t.I + (wave >> 1), cb = 2 * t.J + (wave & 1);        // this wave's 32 x 32 in the end
@@ -396,14 +399,18 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
     // element (row, k) of an operand with KB blocks of 16 k
     auto at = [](int row, int k, int KB) { return (int)frag_at(row >> 5, k >> 4, KB) + ((row & 31) + 32 * ((k >> 3) & 1)) * 8 + (k & 7); };
     auto set = [&](f16* to, int i, float v) { f16 a, b; split(v, a, b); to[i] = a; to[i + FRAG] = b; };
+    T raw[EACH];                                // (clamped addresses and no branch: all of them on their way at once)
     float v[EACH];
     double ss = 0.;
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
+        const int e = threadIdx.x + 256 * i, r = min(p.tall ? e % 64 : e / NP, m - 1), col = min(p.tall ? e / 64 : e % NP, n - 1);
+        raw[i] = g[p.tall ? col * m + r : r * n + col];
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
         const int e = threadIdx.x + 256 * i, r = p.tall ? e % 64 : e / NP, col = p.tall ? e / 64 : e % NP;
-        const bool in = r < m && col < n;
-        const float x = (float)g[in ? (p.tall ? col * m + r : r * n + col) : 0];
-        v[i] = in ? x : 0.f;
+        v[i] = r < m && col < n ? (float)raw[i] : 0.f;
         ss += (double)v[i] * (double)v[i];
     }
     for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
@@ -418,11 +425,11 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
         set(XT, at(col, r, 4), x);
     }
     __syncthreads();
-    // 32 x 32 of P Q^T at fragment row rb and column cb
-    auto product = [&](const f16* P, const f16* Q, int rb, int cb, int KB) {
+    // 32 x 32 of P Q^T at fragment row rb and column cb; what is padding of K alone is left out
+    auto product = [&](const f16* P, const f16* Q, int rb, int cb, int KB, int k) {
         float16v acc = {};
 #pragma unroll 4
-        for (int kb = 0; kb < KB; kb++) {
+        for (int kb = 0; kb < (k + 15) / 16; kb++) {
             const f16 *a = P + frag_at(rb, kb, KB) + lane * 8, *b = Q + frag_at(cb, kb, KB) + lane * 8;
             const half8 ph = *(const half8*)a, pl = *(const half8*)(a + FRAG), qh = *(const half8*)b, ql = *(const half8*)(b + FRAG);
             acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
@@ -432,32 +439,37 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
         return acc;
     };
     // beta S + gamma acc into D^T (laid out like S), its values kept
-    auto finish = [&](float16v& acc, const f16* S, f16* D, int rb, int cb, int MB, float beta, float gamma) {
+    auto finish = [&](float16v& acc, const Summand& s, f16* D, int rb, int cb, int MB, float beta, float gamma) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const long to = place(rb, cb, k, MB);
-            half4 hi = {}, lo = {};
-            if (S) { hi = *(const half4*)(S + to); lo = *(const half4*)(S + to + FRAG); }
+            half4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                acc[4 * k + i] = fmaf(gamma, acc[4 * k + i], beta * ((float)hi[i] + (float)lo[i]));
+                acc[4 * k + i] = fmaf(gamma, acc[4 * k + i], beta * ((float)s.hi[k][i] + (float)s.lo[k][i]));
                 f16 a, b; split(acc[4 * k + i], a, b); hi[i] = a; lo[i] = b;
             }
-            *(half4*)(D + to) = hi; *(half4*)(D + to + FRAG) = lo;
+            f16* to = D + place(rb, cb, k, MB);
+            *(half4*)to = hi; *(half4*)(to + FRAG) = lo;
         }
     };
     const int rb = wave >> 1, cb = wave & 1;
     for (int it = 0; it < steps; it++) {
-        float16v acc = product(X, X, rb, cb, NP / 16);
-        finish(acc, nullptr, A, rb, cb, 4, 0.f, UNSCALE);
+        Summand none = {}, sum, sums[NB];
+        float16v acc = product(X, X, rb, cb, NP / 16, n);
+        finish(acc, none, A, rb, cb, 4, 0.f, UNSCALE);
+#pragma unroll
+        for (int j = 0; j < NB; j++) fetch_summand(sums[j], X, rb + 2 * j, cb, NP / 16);
         __syncthreads();
-        acc = product(A, A, rb, cb, 4);
-        finish(acc, A, B, rb, cb, 4, NS_B, NS_C * UNSCALE);
+        fetch_summand(sum, A, rb, cb, 4);
+        acc = product(A, A, rb, cb, 4, m);
+        finish(acc, sum, B, rb, cb, 4, NS_B, NS_C * UNSCALE);
         __syncthreads();
         // X^T B, NP x 64: blocks rb + 2 j of its rows; X is each lane's own to replace, X^T only when every wave has read it
         float16v next[NB];
 #pragma unroll
-        for (int j = 0; j < NB; j++) { next[j] = product(XT, B, rb + 2 * j, cb, 4); finish(next[j], X, X, rb + 2 * j, cb, NP / 16, NS_A, UNSCALE); }
+        for (int j = 0; j < NB; j++) next[j] = product(XT, B, rb + 2 * j, cb, 4, m);
+#pragma unroll
+        for (int j = 0; j < NB; j++) finish(next[j], sums[j], X, rb + 2 * j, cb, NP / 16, NS_A, UNSCALE);
         __syncthreads();
         if (it + 1 == steps) {                  // (A and B are free: the way to the result)
 #pragma unroll
