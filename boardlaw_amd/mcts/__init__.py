@@ -729,7 +729,9 @@ class _GraphedMove:
             generator = getattr(agent.kwargs.get('rng'), 'generator', None)
             if generator is not None:
                 self.graph.register_generator_state(generator)      # a private generator's offsets must be graph-managed too
-            with torch.cuda.graph(self.graph):
+            # thread_local: the watchdog thread of an nccl process group asks its events whether past collectives are done whenever it likes;
+            # under the default (global) mode such a query from another thread during the capture fails and ends the process
+            with torch.cuda.graph(self.graph, capture_error_mode='thread_local'):
                 self.out = run()
             # what this capture keeps alive -- the tree, its scratch, the block of uniforms: a capture allocates from a pool of
             # its own, so the allocator's reserved bytes grow by exactly that pool (measured, not estimated from shapes)
