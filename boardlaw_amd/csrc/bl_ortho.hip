@@ -438,14 +438,14 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
         }
         return acc;
     };
-    // beta S + gamma acc into D^T (laid out like S), its values kept
-    auto finish = [&](float16v& acc, const Summand& s, f16* D, int rb, int cb, int MB, float beta, float gamma) {
+    // beta s + gamma acc into D^T, its values kept.  The summands are the same lane's values of the product before, in f32
+    auto finish = [&](float16v& acc, const float16v& s, f16* D, int rb, int cb, int MB, float beta, float gamma) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             half4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                acc[4 * k + i] = fmaf(gamma, acc[4 * k + i], beta * ((float)s.hi[k][i] + (float)s.lo[k][i]));
+                acc[4 * k + i] = fmaf(gamma, acc[4 * k + i], beta * s[4 * k + i]);
                 f16 a, b; split(acc[4 * k + i], a, b); hi[i] = a; lo[i] = b;
             }
             f16* to = D + place(rb, cb, k, MB);
@@ -453,23 +453,27 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
         }
     };
     const int rb = wave >> 1, cb = wave & 1;
-    for (int it = 0; it < steps; it++) {
-        Summand none = {}, sum, sums[NB];
-        float16v acc = product(X, X, rb, cb, NP / 16, n);
-        finish(acc, none, A, rb, cb, 4, 0.f, UNSCALE);
+    float16v x[NB];                             // this lane's entries of X^T
 #pragma unroll
-        for (int j = 0; j < NB; j++) fetch_summand(sums[j], X, rb + 2 * j, cb, NP / 16);
+    for (int j = 0; j < NB; j++) {
+        Summand s;
+        fetch_summand(s, X, rb + 2 * j, cb, NP / 16);
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[j][i] = (float)s.hi[i / 4][i % 4] + (float)s.lo[i / 4][i % 4];
+    }
+    for (int it = 0; it < steps; it++) {
+        float16v a = product(X, X, rb, cb, NP / 16, n);
+        finish(a, a, A, rb, cb, 4, 0.f, UNSCALE);
         __syncthreads();
-        fetch_summand(sum, A, rb, cb, 4);
-        acc = product(A, A, rb, cb, 4, m);
-        finish(acc, sum, B, rb, cb, 4, NS_B, NS_C * UNSCALE);
+        float16v b = product(A, A, rb, cb, 4, m);
+        finish(b, a, B, rb, cb, 4, NS_B, NS_C * UNSCALE);
         __syncthreads();
         // X^T B, NP x 64: blocks rb + 2 j of its rows; X is each lane's own to replace, X^T only when every wave has read it
         float16v next[NB];
 #pragma unroll
         for (int j = 0; j < NB; j++) next[j] = product(XT, B, rb + 2 * j, cb, 4, m);
 #pragma unroll
-        for (int j = 0; j < NB; j++) finish(next[j], sums[j], X, rb + 2 * j, cb, NP / 16, NS_A, UNSCALE);
+        for (int j = 0; j < NB; j++) { finish(next[j], x[j], X, rb + 2 * j, cb, NP / 16, NS_A, UNSCALE); x[j] = next[j]; }
         __syncthreads();
         if (it + 1 == steps) {                  // (A and B are free: the way to the result)
 #pragma unroll
