@@ -186,8 +186,8 @@ int bl_abi_version(void) { return 4; }
 const char* bl_strerror(int code) {
     switch (code) {
         case BL_OK: return "ok";
-        case BL_EINVAL: return "invalid argument (null pointer or non-positive size)";
-        case BL_ETOOBIG: return "size beyond kernel limits (A <= 1024, T <= 32767, S <= 8, boardsize <= 32)";
+        case BL_EINVAL: return "invalid argument (null or misaligned pointer, non-positive size, unknown type)";
+        case BL_ETOOBIG: return "size beyond kernel limits (search and board kernels: A <= 1024, T <= 32767, S <= 8, boardsize <= 32; the learner's operators: BL_*_MAX)";
         case BL_ELAUNCH: return "HIP kernel launch failed";
         default: return "unknown error";
     }

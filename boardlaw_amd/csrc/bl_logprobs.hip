@@ -528,7 +528,7 @@ template <typename T> int run(const Grads& q, hipStream_t s) {
 int check_rows(const void* raw, int dtype, long raw_stride, const uint8_t* valid, long valid_stride, long R, int A, int k) {
     if (!raw || R <= 0 || A <= 0 || k < 0 || raw_stride < 0 || (valid && valid_stride < 0)) return BL_EINVAL;
     if (dtype != BL_F32 && dtype != BL_F16 && dtype != BL_BF16) return BL_EINVAL;
-    if (k > BL_TOP_MAX || A > (1 << 30) || R > (1l << 24)) return BL_ETOOBIG;      // (the largest grid: 2^24 rows x 64 lanes or parts)
+    if (k > BL_TOP_MAX || A > BL_LOGPROBS_MAX || R > BL_LOGPROBS_ROWS) return BL_ETOOBIG;      // (the largest grid: 2^24 rows x 64 lanes)
     return BL_OK;
 }
 
@@ -548,7 +548,7 @@ int bl_logprobs(const void* raw, int dtype, long raw_stride, const uint8_t* vali
     if (const int rc = check_rows(raw, dtype, raw_stride, valid, valid_stride, R, A, k)) return rc;
     if (!entropy || (actions == nullptr) != (logp == nullptr) || (k > 0 && (!top || !top_logp))) return BL_EINVAL;
     Rows q{raw, raw_stride, valid, valid_stride, actions, R, A, k, logp, entropy, top, top_logp, stats, parts_of(R, A), (char*)workspace};
-    if (q.S > 1 && !workspace) return BL_EINVAL;
+    if (q.S > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7))) return BL_EINVAL;
     const hipStream_t s = (hipStream_t)stream;
     return dtype == BL_F32 ? run<float>(q, s) : dtype == BL_F16 ? run<f16>(q, s) : run<bf16>(q, s);
 }

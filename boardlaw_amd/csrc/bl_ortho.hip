@@ -387,18 +387,31 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
 }
 
 // ---- m <= 64 and n <= 64 NB: one workgroup takes a matrix through all of it in LDS ------------------------------------------------------
-// 15 dependent products of a few hundred cycles each: launches (3 to 5 us apiece) would be nearly all of the time.
+// 15 dependent products of a few hundred cycles each: launches (3 to 5 us apiece) would be nearly all of the time.  Here products cost next
+// to nothing, so operands are three f16 numbers (33 bits) and a product six: a small matrix is often nearly singular, and sums this
+// short leave f32 so little error of their own that 22 bits would show (8 x 8: up to 4.8 times f32's).
+constexpr int TRIPLE = 3 * FRAG;
+__device__ __forceinline__ int triple_at(int rb, int kb, int KB) { return (rb * KB + kb) * TRIPLE; }
+__device__ __forceinline__ void split(float v, f16 (&o)[3]) {
+    o[0] = (f16)v;
+    const float r = v - (float)o[0];
+    o[1] = (f16)r;
+    o[2] = (f16)(r - (float)o[1]);
+}
 template <typename T, int NB>
 __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int steps, float eps) {
     extern __shared__ __align__(16) char smem[];
     __shared__ double sums[4];
     constexpr int NP = 64 * NB, EACH = 64 * NP / 256;
-    f16 *X = (f16*)smem, *XT = X + 2 * 64 * NP, *A = XT + 2 * 64 * NP, *B = A + 2 * 64 * 64;
+    f16 *X = (f16*)smem, *XT = X + 3 * 64 * NP, *A = XT + 3 * 64 * NP, *B = A + 3 * 64 * 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, m = p.m, n = p.n;
     const T* g = (const T*)q.in[blockIdx.x];
     // element (row, k) of an operand with KB blocks of 16 k
-    auto at = [](int row, int k, int KB) { return (int)frag_at(row >> 5, k >> 4, KB) + ((row & 31) + 32 * ((k >> 3) & 1)) * 8 + (k & 7); };
-    auto set = [&](f16* to, int i, float v) { f16 a, b; split(v, a, b); to[i] = a; to[i + FRAG] = b; };
+    auto set = [&](f16* to, int row, int k, int KB, const f16 (&s)[3]) {
+        to += triple_at(row >> 5, k >> 4, KB) + ((row & 31) + 32 * ((k >> 3) & 1)) * 8 + (k & 7);
+#pragma unroll
+        for (int i = 0; i < 3; i++) to[i * FRAG] = s[i];
+    };
     T raw[EACH];                                // (clamped addresses and no branch: all of them on their way at once)
     float v[EACH];
     double ss = 0.;
@@ -420,47 +433,61 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
         const int e = threadIdx.x + 256 * i, r = p.tall ? e % 64 : e / NP, col = p.tall ? e / 64 : e % NP;
-        const float x = (float)((double)v[i] * inv);
-        set(X, at(r, col, NP / 16), x);
-        set(XT, at(col, r, 4), x);
+        f16 s[3];
+        split((float)((double)v[i] * inv), s);
+        set(X, r, col, NP / 16, s);
+        set(XT, col, r, 4, s);
     }
     __syncthreads();
     // 32 x 32 of P Q^T at fragment row rb and column cb; what is padding of K alone is left out
     auto product = [&](const f16* P, const f16* Q, int rb, int cb, int KB, int k) {
         float16v acc = {};
-#pragma unroll 4
         for (int kb = 0; kb < (k + 15) / 16; kb++) {
-            const f16 *a = P + frag_at(rb, kb, KB) + lane * 8, *b = Q + frag_at(cb, kb, KB) + lane * 8;
-            const half8 ph = *(const half8*)a, pl = *(const half8*)(a + FRAG), qh = *(const half8*)b, ql = *(const half8*)(b + FRAG);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+            half8 a[3], b[3];
+#pragma unroll
+            for (int i = 0; i < 3; i++) {
+                a[i] = *(const half8*)(P + triple_at(rb, kb, KB) + i * FRAG + lane * 8);
+                b[i] = *(const half8*)(Q + triple_at(cb, kb, KB) + i * FRAG + lane * 8);
+            }
+            // the smallest first; lo mid, mid lo and lo lo are under 2^-33 of the product
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[2], b[0], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[2], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[1], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc, 0, 0, 0);
         }
         return acc;
     };
+    // a lane's 4 consecutive k of D^T, group `k`
+    auto spot = [&](int rb, int cb, int k, int MB) { return triple_at(cb, 2 * rb + (k >> 1), MB) + (c + 32 * (k & 1)) * 8 + 4 * h; };
     // beta s + gamma acc into D^T, its values kept.  The summands are the same lane's values of the product before, in f32
     auto finish = [&](float16v& acc, const float16v& s, f16* D, int rb, int cb, int MB, float beta, float gamma) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            half4 hi, lo;
+            half4 o[3];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 acc[4 * k + i] = fmaf(gamma, acc[4 * k + i], beta * s[4 * k + i]);
-                f16 a, b; split(acc[4 * k + i], a, b); hi[i] = a; lo[i] = b;
+                f16 t[3];
+                split(acc[4 * k + i], t);
+                o[0][i] = t[0]; o[1][i] = t[1]; o[2][i] = t[2];
             }
-            f16* to = D + place(rb, cb, k, MB);
-            *(half4*)to = hi; *(half4*)(to + FRAG) = lo;
+#pragma unroll
+            for (int i = 0; i < 3; i++) *(half4*)(D + spot(rb, cb, k, MB) + i * FRAG) = o[i];
         }
     };
     const int rb = wave >> 1, cb = wave & 1;
     float16v x[NB];                             // this lane's entries of X^T
 #pragma unroll
-    for (int j = 0; j < NB; j++) {
-        Summand s;
-        fetch_summand(s, X, rb + 2 * j, cb, NP / 16);
+    for (int j = 0; j < NB; j++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[j][i] = (float)s.hi[i / 4][i % 4] + (float)s.lo[i / 4][i % 4];
-    }
+        for (int k = 0; k < 4; k++) {
+            const f16* from = X + spot(rb + 2 * j, cb, k, NP / 16);
+            const half4 hi = *(const half4*)from, mid = *(const half4*)(from + FRAG), lo = *(const half4*)(from + 2 * FRAG);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[j][4 * k + i] = (float)hi[i] + ((float)mid[i] + (float)lo[i]);
+        }
     for (int it = 0; it < steps; it++) {
         float16v a = product(X, X, rb, cb, NP / 16, n);
         finish(a, a, A, rb, cb, 4, 0.f, UNSCALE);
@@ -488,7 +515,11 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
 #pragma unroll
         for (int j = 0; j < NB; j++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) set(XT, at(32 * (rb + 2 * j) + 8 * (i >> 2) + 4 * h + (i & 3), 32 * cb + c, 4), next[j][i]);
+            for (int i = 0; i < 16; i++) {
+                f16 s[3];
+                split(next[j][i], s);
+                set(XT, 32 * (rb + 2 * j) + 8 * (i >> 2) + 4 * h + (i & 3), 32 * cb + c, 4, s);
+            }
         __syncthreads();
     }
 }
@@ -519,7 +550,7 @@ template <int MODE> bool multiply(const Product& p, const Mats& q, hipStream_t s
 }
 
 template <typename T, int NB> bool small(const Product& p, const Mats& q, int steps, float eps, hipStream_t s) {
-    constexpr size_t bytes = 2 * sizeof(f16) * (2 * 64 * 64 * NB + 2 * 64 * 64);
+    constexpr size_t bytes = 3 * sizeof(f16) * (2 * 64 * 64 * NB + 2 * 64 * 64);
     static size_t raised[64];
     if (!bl_raise_lds_limit((const void*)ortho_small_kernel<T, NB>, bytes, raised)) return false;
     hipLaunchKernelGGL((ortho_small_kernel<T, NB>), dim3(p.count), dim3(256), bytes, s, q, p, steps, eps);
@@ -568,6 +599,7 @@ int bl_orthogonalize(const void* const* host_in, void* const* host_out, int coun
     if (!host_in || !host_out || !workspace || count <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || !(eps >= 0.f)) return BL_EINVAL;
     if (dtype != BL_F32 && dtype != BL_F16 && dtype != BL_BF16) return BL_EINVAL;
     if (rows > BL_ORTHO_MAX || cols > BL_ORTHO_MAX) return BL_ETOOBIG;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return BL_EINVAL;
     for (int i = 0; i < count; i++) if (!host_in[i] || !host_out[i]) return BL_EINVAL;
     const hipStream_t s = (hipStream_t)stream;
     const int tall = rows > cols, m = tall ? cols : rows, n = tall ? rows : cols;

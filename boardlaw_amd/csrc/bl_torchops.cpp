@@ -121,6 +121,7 @@ py::tuple py_logprobs(const Tensor& raw, const Maybe& actions, const Maybe& vali
     device_check(raw, {&actions, &valid});
     const auto lead = raw.sizes().slice(0, raw.dim() - 1);
     const int64_t A = raw.size(-1);
+    value_check(A <= BL_LOGPROBS_MAX && raw.numel() / A <= BL_LOGPROBS_ROWS, "up to ", BL_LOGPROBS_ROWS, " rows of up to ", BL_LOGPROBS_MAX, " moves are supported, got ", shape_of(raw.sizes()));
     const Tensor flat = rows_of(raw, A);
     Maybe a, v;
     if (actions) {

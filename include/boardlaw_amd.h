@@ -409,7 +409,7 @@ int bl_sim_expand_counted(const bl_search_t* s, int sim, const void* rands, int1
 #define BL_F16 1
 #define BL_BF16 2
 
-/* Log probabilities of given moves, entropy and the best alternatives of R rows of A unnormalised logits (A <= 2^30, R <= 2^24).
+/* Log probabilities of given moves, entropy and the best alternatives of R <= BL_LOGPROBS_ROWS rows of A <= BL_LOGPROBS_MAX unnormalised logits.
  * valid (R,A) u8 or NULL: entries with 0 count as logits of -inf, whatever raw holds there; an entry of -inf has probability 0, is never an
  * alternative, and its gradient is 0.  Per row, with log p = log_softmax:
  *   logp_out[r] = log p[actions[r]]: -inf for an entry of probability 0; 0 if actions[r] < 0 (no move given); NaN if actions[r] >= A.
@@ -422,6 +422,8 @@ int bl_sim_expand_counted(const bl_search_t* s, int sim, const void* rands, int1
  * the best alternative).  workspace: bl_logprobs_workspace(R, A, k) bytes, 8-byte aligned (0: may be NULL).  All sums in f32, in an order
  * that depends on the arguments only. */
 #define BL_TOP_MAX 64
+#define BL_LOGPROBS_MAX (1 << 30)
+#define BL_LOGPROBS_ROWS (1 << 24)
 long bl_logprobs_workspace(long R, int A, int k);
 int bl_logprobs(const void* raw, int dtype, long raw_stride, const uint8_t* valid, long valid_stride, const long long* actions /*i64 (R)*/,
                 long R, int A, int k, float* logp_out /*(R)*/, float* entropy_out /*(R)*/, long long* top_out, float* top_logp_out,

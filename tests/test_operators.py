@@ -607,6 +607,45 @@ def test_a_learner_with_all_of_them(block):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('precision', ['fp16', 'fp32'])
+def test_gated_network_in_a_search(precision):
+    """A search on a gated network's inference plan, eager and captured: the same moves; a plan follows its module's weights."""
+    from boardlaw_amd import hex, networks
+    from boardlaw_amd.mcts import MCTSAgent
+    worlds = hex.Hex.initial(16, 4)
+    torch.manual_seed(1)
+    net = networks.FCModel(worlds.obs_space, worlds.action_space, width=40, depth=2, block='gated').cuda()
+    with torch.no_grad():
+        for b in list(net.body)[1:]:
+            getattr(b, 'α').fill_(.5)
+    plan = networks.Inference(net, precision=precision)
+    seen = []
+    for graph in (False, True):
+        agent = MCTSAgent(plan, n_nodes=8, graph=graph)
+        agent(worlds)
+        torch.manual_seed(3)
+        seen.append(agent(worlds))
+    assert torch.equal(seen[0].actions, seen[1].actions) and torch.equal(seen[0].logits, seen[1].logits)
+    before = plan.root_raw(worlds)[0].clone()
+    with torch.no_grad():
+        net.body[1].post.mul_(2.)
+    assert not torch.equal(before, plan.root_raw(worlds)[0])
+
+
+@pytest.mark.gpu
+def test_single_rows():
+    """One row without leading dimensions."""
+    from boardlaw_amd import heads, networks
+    x = torch.randn(81, device='cuda')
+    out = heads.logprobs(x, torch.tensor(3, device='cuda'), x > 0, k=2)
+    two = heads.logprobs(x[None], torch.tensor([3], device='cuda'), (x > 0)[None], k=2)
+    assert out.logp.shape == () and out.top.shape == (2,) and all(torch.equal(a, b[0]) for a, b in zip(out.values(), two.values()))
+    y, w = torch.randn(162, device='cuda'), torch.ones(81, device='cuda')
+    a, b = networks.norm_residual(x, y, None, w, pre=w), networks.norm_residual(x[None], y[None], None, w, pre=w)
+    assert a[0].shape == a[1].shape == (81,) and torch.equal(a[0], b[0][0]) and torch.equal(a[1], b[1][0])
+
+
+@pytest.mark.gpu
 def test_head_evaluates_without_the_rows():
     from boardlaw_amd import heads
     torch.manual_seed(0)
