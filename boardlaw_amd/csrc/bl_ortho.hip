@@ -350,15 +350,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
         put(r[free], free);
         fetch(r[free], s + 7);
         multiply_add<F>(f[slot & 1], acc);
+        // what LDS does comes first, so that the barrier finds it done; the loads go under the last products
 #pragma unroll
-        for (int i = 0; i < 2 * NL; i++) {                  // reads first, writes and loads in turn behind them, products throughout
+        for (int i = 0; i < NL; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if constexpr (F == 4) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (i & 1) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, F == 4 ? 1 : 0, 0);
-            if (i & 1) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 6 * F, 0);
+#pragma unroll
+        for (int i = 0; i < NL; i++) { __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
         __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
     };
