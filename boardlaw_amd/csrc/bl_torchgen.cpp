@@ -1,4 +1,4 @@
-// bl_torchgen.cpp -- libbl_torchgen.so: the one place where this package touches a torch C++ type.
+// bl_torchgen.cpp -- libbl_torchgen.so: torch's generator state (one of two places where this package touches torch C++ types; bl_torchops.cpp is the other).
 //
 // The reference draws its descend uniforms with at::rand_like from torch's generator (boardlaw/mcts/cpp/cuda.cu:191), T-1 times
 // per move.  bl_rand_block (libboardlaw_amd.so, torch-free) reproduces those T-1 draws with one launch; to stay on the
