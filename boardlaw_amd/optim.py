@@ -72,6 +72,19 @@ class Muon(torch.optim.Optimizer):
         return loss
 
 
+class Several(tuple):
+    """Optimisers that share a network's parameters out among them, as training.optimize takes them; saved and loaded as one (storage.save(opt=...))."""
+
+    def state_dict(self):
+        return {str(i): o.state_dict() for i, o in enumerate(self)}
+
+    def load_state_dict(self, state):
+        if len(state) != len(self):
+            raise ValueError(f'a state of {len(state)} optimisers for {len(self)}')
+        for i, o in enumerate(self):
+            o.load_state_dict(state[str(i)])
+
+
 def split(network):
     """A network's parameters as (hidden weight matrices, the rest): the residual blocks' weights are Muon's, biases, gains, the intake
     and the heads Adam's."""

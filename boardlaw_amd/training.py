@@ -82,7 +82,7 @@ def make_optimizer(network, optimizer='adam', lr=1e-3, hidden_lr=0.02):
     hidden, rest = optim.split(network)
     if not hidden:
         raise ValueError('the network has no residual blocks for Muon')
-    return optim.Muon(hidden, lr=hidden_lr), torch.optim.Adam(rest, lr=lr)
+    return optim.Several((optim.Muon(hidden, lr=hidden_lr), torch.optim.Adam(rest, lr=lr)))
 
 
 def run(worlds, network, n_steps, nodes=64, c_puct=1 / 16, lr=1e-3, buffer_len=64, graph=False, inference=None, on_step=None, timings=None,

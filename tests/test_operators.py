@@ -633,6 +633,36 @@ def test_gated_network_in_a_search(precision):
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Tensors of more than 2^31 elements: their last rows are computed and written where they are."""
+    from boardlaw_amd import heads, networks
+    R, A = 70000, 32768
+    raw = torch.zeros((R, A), dtype=torch.bfloat16, device='cuda')
+    raw[-3:] = torch.randn((3, A), device='cuda').bfloat16()
+    actions = torch.full((R,), A - 1, device='cuda')
+    tail = raw[-3:].clone().requires_grad_()
+    want = heads.logprobs(tail, actions[-3:], k=3)
+    raw.requires_grad_()
+    got = heads.logprobs(raw, actions, k=3)
+    # (another number of waves per row: other roundings)
+    assert torch.equal(got.top[-3:], want.top) and torch.allclose(got.entropy[-3:], want.entropy, rtol=200 * U) and torch.allclose(got.logp[-3:], want.logp, rtol=200 * U)
+    # equal entries: c of them and nothing else, log s one rounding of log A off
+    assert torch.allclose(got.entropy[:-3].double(), torch.full((), math.log(A), dtype=torch.float64, device='cuda'), rtol=4 * U, atol=0)
+    d, = torch.autograd.grad(got.logp.sum(), raw)
+    e, = torch.autograd.grad(want.logp.sum(), tail)
+    assert torch.allclose(d[-3:].float(), e.float(), rtol=4 * half_step(torch.bfloat16), atol=1e-12)
+    assert (d[::9000, -1] > .9).all()
+    del raw, got, d
+    R, W = 270000, 8192
+    x = torch.zeros((R, W), dtype=torch.float16, device='cuda')
+    x[-2:] = torch.randn((2, W), device='cuda').half()
+    pre = torch.rand(W, device='cuda')
+    out, h = networks.norm_residual(x, x, None, pre, None, pre)
+    o2, h2 = networks.norm_residual(x[-2:].clone(), x[-2:].clone(), None, pre, None, pre)
+    assert torch.equal(out[-2:], o2) and torch.equal(h[-2:], h2) and (out[:4] == 0).all() and (h[R - 3] == 0).all()
+
+
+@pytest.mark.gpu
 def test_single_rows():
     """One row without leading dimensions."""
     from boardlaw_amd import heads, networks
@@ -701,6 +731,23 @@ def test_refusals():
     muon, adam = training.make_optimizer(net, 'muon')
     assert {id(p) for o in (muon, adam) for g in o.param_groups for p in g['params']} == {id(p) for p in net.parameters()}
     assert [tuple(p.shape) for p in muon.param_groups[0]['params']] == [(16, 16)] * 2
+
+
+def test_several_optimisers_are_saved_as_one(tmp_path):
+    from boardlaw_amd import heads, networks, storage, training
+    net = networks.FCModel(heads.Tensor((3, 3, 2)), heads.Masked(9), width=16, depth=2)
+    opts = training.make_optimizer(net, 'muon', lr=.5, hidden_lr=.25)
+    for p in net.parameters():
+        p.grad = torch.ones_like(p)
+    opts[1].step()
+    storage.save(tmp_path / 'x', agent=net, opt=opts)
+    state = storage.load(tmp_path / 'x')['opt']
+    other = training.make_optimizer(net, 'muon')
+    other.load_state_dict(state)
+    assert [o.param_groups[0]['lr'] for o in other] == [.25, .5]
+    assert torch.equal(other[1].state[net.policy.core.weight]['exp_avg'], opts[1].state[net.policy.core.weight]['exp_avg'])
+    with pytest.raises(ValueError):
+        other.load_state_dict({'0': state['0']})
 
 
 @pytest.mark.gpu
