@@ -6,10 +6,10 @@
 //     z  = g_x' + rx (t - xn mean(t xn)),  t = g_h pre;      dx = z;      dpre = sum_rows g_h xn;      dalpha = sum z u
 //     dgate = alpha z post n s (1 - s);    dpost = sum_rows alpha z s n;  dy = ry (dn - n mean(dn n)),  dn = alpha z s post
 // Everything is computed in f32 and rounded once at its store.  The bound is HBM: every element is read once and written once; a row
-// is held in registers by G lanes of N elements each, so the two dependent sums of a row cost no second read.  The sums over rows are
+// is held in registers by G lanes of 8 elements each, so the two dependent sums of a row cost no second read.  The sums over rows are
 // kept per workgroup in registers over all of its rows and added up by a second launch in a fixed order: no atomics, the same bits
-// every time.  32768 x 512, f32 stream, f16 branches with gates: forward 42 us for 235 MB (5.5 TB/s), backward 67 us for 369 MB (5.5 TB/s) and
-// 4 us for the sums; 8192 x 4096 bf16 forward 58 us for 335 MB (5.8 TB/s); a copy of 4 GiB runs at 4.75 TB/s, of 32 MiB at 6.6.
+// every time.  32768 x 512, f32 stream, f16 branches with gates: forward 42 us for 235 MB (5.5 TB/s), backward 68 us for 369 MB (5.4 TB/s) and
+// 4 us for the sums; 4096 x 771 f32 14 + 21 + 4 us; 8192 x 4096 bf16 forward 58 us for 335 MB (5.8 TB/s); a copy of 4 GiB runs at 4.75 TB/s, of 32 MiB at 6.6.
 #include "bl_train.h"
 
 #pragma clang fp contract(off)
@@ -29,6 +29,13 @@ struct Norm {
     const void* gx; long gxs; const void* gh; long ghs;          // backward
     void* dx; void* dy; long dys; void* dgate; long dgs; float* parts;
 };
+
+// which of a workgroup's rows: the same for a wave's lanes where a row is a wave's or more, and said so, which makes a row's addresses scalar
+template <int G> __device__ __forceinline__ int group_of() {
+    const int g = threadIdx.x / G;
+    if constexpr (G >= 64) return __builtin_amdgcn_readfirstlane(g);
+    return g;
+}
 
 // where lane gl's N elements of a row are: VEC == 8 in eights (16-byte accesses), VEC == 1 every G-th
 template <int G, int VEC> __device__ __forceinline__ int column(int gl, int i) { return VEC == 8 ? 8 * (gl + G * (i / 8)) + i % 8 : gl + G * i; }
@@ -69,8 +76,8 @@ template <int G, int VEC, typename T, int N> __device__ __forceinline__ void wri
     }
 }
 
-// sum over the G lanes of a row, in every one of them.  G > 64: the row is a workgroup's; `lds` holds a value per wave, two sets of
-// them in turn (`set`), so that one barrier per sum is enough
+// sum over the G lanes of a row, in every one of them.  G > 64: a row is several waves'; `lds` holds a value per wave, two sets of them in
+// turn (`set`), so that one barrier per sum is enough
 template <int G> __device__ __forceinline__ float row_sum(float v, float* lds, int& set) {
     v = reduce<(G < 64 ? G : 64), Sum>(v);
     if constexpr (G > 64) {
@@ -78,6 +85,7 @@ template <int G> __device__ __forceinline__ float row_sum(float v, float* lds, i
         set ^= 1;
         if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
         __syncthreads();
+        at += threadIdx.x / G * (G / 64);
         v = at[0];
 #pragma unroll
         for (int w = 1; w < G / 64; w++) v += at[w];
@@ -98,23 +106,18 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(Norm q) {
     const int gl = threadIdx.x & (G - 1);
     int set = 0;
     float post[N], pre[N], gate[N];
-    constexpr bool KEEP = N == 8;           // gains in registers for all rows; 16 elements per lane leave no room, and a row's are read with it
-    auto gains = [&] {
-        if (q.post) read<G, VEC>(q.post, gl, q.W, post);
-        if (q.pre) read<G, VEC>(q.pre, gl, q.W, pre);
-        if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
-    };
-    if constexpr (KEEP) gains();
+    if (q.post) read<G, VEC>(q.post, gl, q.W, post);
+    if (q.pre) read<G, VEC>(q.pre, gl, q.W, pre);
+    if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
     const float alpha = q.alpha ? *q.alpha : 1.f;
     for (long r0 = (long)blockIdx.x * ROWS; r0 < q.R; r0 += (long)gridDim.x * ROWS) {
-        const long row = r0 + threadIdx.x / G, at = row < q.R ? row : q.R - 1;      // (G > 64: one row per workgroup, always live)
+        const long row = r0 + group_of<G>(), at = row < q.R ? row : q.R - 1;      // (G > 64: one row per workgroup, always live)
         const bool live = row < q.R;
         Elements<G, VEC, N, TX> ex;
         Elements<G, VEC, N, TY> ey, eg;
         ex.fetch((const TX*)q.x + at * q.xs, gl, q.W);
         if (q.y) ey.fetch((const TY*)q.y + at * q.ys, gl, q.W);
         if (q.kind == BL_GATE_FULL) eg.fetch((const TY*)q.gate + at * q.gs, gl, q.W);
-        if constexpr (!KEEP) gains();
         float x[N];
         ex.get(x, gl, q.W);
         float ry = 1.f;
@@ -161,23 +164,26 @@ template <typename TX, typename TY, int G, int N, int VEC>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
     __shared__ float lds[32];
     constexpr int T = G > 256 ? G : 256, ROWS = T / G;
-    __shared__ float cols[G <= 64 ? 3 * N * G + 1 : 1];
+    __shared__ float cols[ROWS > 1 ? 3 * N * G + 1 : 1];
     const int gl = threadIdx.x & (G - 1);
     int set = 0;
     float post[N], pre[N], gate[N];
-    constexpr bool KEEP = N == 8;           // gains in registers for all rows; 16 elements per lane leave no room, and a row's are read with it
+    constexpr bool KEEP = G < 1024;         // gains in registers for all rows; a workgroup of 16 waves has no room, and a row's are read with it
     auto gains = [&] {
         if (q.post) read<G, VEC>(q.post, gl, q.W, post);
         if (q.gh) read<G, VEC>(q.pre, gl, q.W, pre);
         if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
     };
+    if (!q.post)
+#pragma unroll
+        for (int i = 0; i < N; i++) post[i] = 1.f;
     if constexpr (KEEP) gains();
     const float alpha = q.alpha ? *q.alpha : 1.f;
     float spost[N], spre[N], sgate[N], salpha = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i++) spost[i] = spre[i] = sgate[i] = 0.f;
     for (long r0 = (long)blockIdx.x * ROWS; r0 < q.R; r0 += (long)gridDim.x * ROWS) {
-        const long row = r0 + threadIdx.x / G, at = row < q.R ? row : q.R - 1;
+        const long row = r0 + group_of<G>(), at = row < q.R ? row : q.R - 1;
         const bool live = row < q.R;
         const float ry = q.stats[2 * at], rx = q.stats[2 * at + 1];
         Elements<G, VEC, N, TX> ex, ez;
@@ -188,7 +194,8 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
         if (q.gx) ez.fetch((const TX*)q.gx + at * q.gxs, gl, q.W);
         if (q.gh) et.fetch((const TY*)q.gh + at * q.ghs, gl, q.W);
         if constexpr (!KEEP) gains();
-        float x[N], z[N], n[N], s[N], ds[N], u[N], t[N];
+        // (beyond W everything is 0, so nothing there counts; the sigmoid is computed twice rather than held)
+        float x[N], z[N], n[N];
         ex.get(x, gl, q.W);
         if (q.y) {
             ey.get(n, gl, q.W);
@@ -198,30 +205,26 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
 #pragma unroll
                 for (int i = 0; i < N; i++) gate[i] = g;
             }
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                n[i] *= ry;
+                const float u = post[i] * n[i];
+                x[i] = fmaf(alpha, q.kind != BL_GATE_NONE ? u * sigmoid(gate[i]).s : u, x[i]);
+            }
         }
         if (q.gx) ez.get(z, gl, q.W);
         else
 #pragma unroll
             for (int i = 0; i < N; i++) z[i] = 0.f;
-        if (q.gh) et.get(t, gl, q.W);
-        if (q.y) {
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                n[i] *= ry;
-                u[i] = q.post ? post[i] * n[i] : n[i];
-                if (q.kind != BL_GATE_NONE) { const Gate g = sigmoid(gate[i]); s[i] = g.s; ds[i] = g.ds; u[i] *= g.s; }
-                else { s[i] = 1.f; ds[i] = 0.f; }
-                x[i] = fmaf(alpha, u[i], x[i]);
-            }
-        }
         if (q.gh) {
-            float c = 0.f;
+            float t[N], c = 0.f;
+            et.get(t, gl, q.W);
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 x[i] *= rx;                                                          // xn
                 if (live) spre[i] = fmaf(t[i], x[i], spre[i]);
                 t[i] *= pre[i];
-                c = column<G, VEC>(gl, i) < q.W ? fmaf(t[i], x[i], c) : c;
+                c = fmaf(t[i], x[i], c);
             }
             c = row_sum<G>(c, lds, set) * q.inv_w;
             // one column: xn^2 = 1 - eps rx^2, and the difference would cancel
@@ -231,17 +234,32 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
         if (live) write<G, VEC>((TX*)q.dx + at * q.W, gl, q.W, z);
         if (!q.y) continue;
         float c = 0.f, cg = 0.f, dn[N];
+        if (q.kind != BL_GATE_NONE) {
+            float dg[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const bool in = column<G, VEC>(gl, i) < q.W;
-            if (live && in) salpha = fmaf(z[i], u[i], salpha);
-            const float v = alpha * z[i], vn = v * n[i], p = q.post ? post[i] : 1.f;
-            dn[i] = v * s[i] * p;
-            if (live) spost[i] = fmaf(vn, s[i], spost[i]);
-            ds[i] *= vn * p;                                                         // dgate
-            if (live) sgate[i] += ds[i];
-            cg += in ? ds[i] : 0.f;
-            c = in ? fmaf(dn[i], n[i], c) : c;
+            for (int i = 0; i < N; i++) {
+                const Gate g = sigmoid(gate[i]);
+                const float v = alpha * z[i], vn = v * n[i], sp = g.s * post[i];
+                if (live) { salpha = fmaf(z[i], n[i] * sp, salpha); spost[i] = fmaf(vn, g.s, spost[i]); }
+                dn[i] = v * sp;
+                c = fmaf(dn[i], n[i], c);
+                dg[i] = vn * post[i] * g.ds;
+                if (live) sgate[i] += dg[i];
+                cg += dg[i];
+            }
+            if (q.kind == BL_GATE_FULL && q.dgate && live) write<G, VEC>((TY*)q.dgate + at * q.dgs, gl, q.W, dg);
+            if (q.kind == BL_GATE_ROW) {
+                cg = row_sum<G>(cg, lds, set);
+                if (q.dgate && live && gl == 0) ((TY*)q.dgate)[at * q.dgs] = (TY)cg;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float v = alpha * z[i];
+                if (live) { salpha = fmaf(z[i], n[i] * post[i], salpha); spost[i] = fmaf(v, n[i], spost[i]); }
+                dn[i] = v * post[i];
+                c = fmaf(dn[i], n[i], c);
+            }
         }
         if (q.post) {
             c = row_sum<G>(c, lds, set) * q.inv_w;
@@ -249,24 +267,17 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
             for (int i = 0; i < N; i++) dn[i] = ry * (q.W == 1 ? dn[i] * (q.eps * ry * ry) : fmaf(-n[i], c, dn[i]));
         }
         if (live) write<G, VEC>((TY*)q.dy + at * q.dys, gl, q.W, dn);
-        if (q.dgate && q.kind == BL_GATE_FULL && live) write<G, VEC>((TY*)q.dgate + at * q.dgs, gl, q.W, ds);
-        if (q.kind == BL_GATE_ROW) {
-            cg = row_sum<G>(cg, lds, set);
-            if (q.dgate && live && gl == 0) ((TY*)q.dgate)[at * q.dgs] = (TY)cg;
-        }
     }
     // this workgroup's sums over its rows: dpost, dpre, dgate per column, then dalpha
     float* out = q.parts + (long)blockIdx.x * (3l * q.W + 1);
     salpha = row_sum<G>(salpha, lds, set);
-    if constexpr (G > 64) {
-        if (T == G) {
+    if constexpr (ROWS == 1) {
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int j = column<G, VEC>(gl, i);
-                if (j < q.W) { out[j] = spost[i]; out[q.W + j] = spre[i]; out[2 * q.W + j] = sgate[i]; }
-            }
-            if (gl == 0) out[3 * q.W] = salpha;
+        for (int i = 0; i < N; i++) {
+            const int j = column<G, VEC>(gl, i);
+            if (j < q.W) { out[j] = spost[i]; out[q.W + j] = spre[i]; out[2 * q.W + j] = sgate[i]; }
         }
+        if (gl == 0) out[3 * q.W] = salpha;
     } else {
         // the workgroup's groups of lanes one after the other: a fixed order
         for (int g = 0; g < ROWS; g++) {
@@ -314,19 +325,21 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(Sums q) {
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------
-// Lanes and elements per lane by width: a row in one wave up to 1024 (no barrier; 4096 x 771 f32 forward + backward 50 us in four waves of 8 elements),
-// a row per 16 lanes up to 128 (four rows to a wave)
-struct Lanes { int G, N; };
-Lanes lanes_of(int W) { return W <= 128 ? Lanes{16, 8} : W <= 512 ? Lanes{64, 8} : W <= 1024 ? Lanes{64, 16} : W <= 2048 ? Lanes{256, 8} : W <= 4096 ? Lanes{512, 8} : Lanes{512, 16}; }
+// Lanes of a row, 8 elements each: the fewest that hold it -- 16 rows to a wave up to 32 wide, a row to a wave up to 512 (no barrier), to a
+// workgroup from 1025 on.  (16 elements per lane need 300 registers in the backward pass: 16384 x 768 f32 114 us with its launches, with 8 per lane in two
+// waves 84.)  Beyond 4096 wide sixteen waves leave a lane 128 registers of the 150 it needs, and what spills bounds the backward pass: 2048 x 8192 f32 / f16 196 us,
+// 1.9 TB/s, where 4096 x 4096 takes 98; the forward pass fits (44 us, 5.4 TB/s)
+constexpr int N = 8;
+int lanes_of(int W) { return W <= 32 ? 4 : W <= 128 ? 16 : W <= 512 ? 64 : W <= 1024 ? 128 : W <= 2048 ? 256 : W <= 4096 ? 512 : 1024; }
 // workgroups of the backward pass: each leaves 3 W + 1 sums, so no more than keep the chip full
 int blocks_of(long R, int W) {
-    const int G = lanes_of(W).G, rows = G > 256 ? 1 : 256 / G;
+    const int G = lanes_of(W), rows = G > 256 ? 1 : 256 / G;
     const long need = (R + rows - 1) / rows, most = 512;
     return (int)(need < most ? need : most);
 }
 bool aligned(const void* p, long stride, int size) { return !p || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * size) % 16 == 0); }
 
-template <typename TX, typename TY, int G, int N, int VEC> int go(const Norm& q, bool grad, hipStream_t s) {
+template <typename TX, typename TY, int G, int VEC> int go(const Norm& q, bool grad, hipStream_t s) {
     constexpr int T = G > 256 ? G : 256, ROWS = T / G;
     if (grad) hipLaunchKernelGGL((norm_grad_kernel<TX, TY, G, N, VEC>), dim3((unsigned)blocks_of(q.R, q.W)), dim3(T), 0, s, q);
     else {
@@ -336,14 +349,14 @@ template <typename TX, typename TY, int G, int N, int VEC> int go(const Norm& q,
     return check_launch();
 }
 template <typename TX, typename TY, int VEC> int by_lanes(const Norm& q, bool grad, hipStream_t s) {
-    const Lanes l = lanes_of(q.W);
-    switch (l.G * l.N) {
-        case 128: return go<TX, TY, 16, 8, VEC>(q, grad, s);
-        case 512: return go<TX, TY, 64, 8, VEC>(q, grad, s);
-        case 1024: return go<TX, TY, 64, 16, VEC>(q, grad, s);
-        case 2048: return go<TX, TY, 256, 8, VEC>(q, grad, s);
-        case 4096: return go<TX, TY, 512, 8, VEC>(q, grad, s);
-        default: return go<TX, TY, 512, 16, VEC>(q, grad, s);
+    switch (lanes_of(q.W)) {
+        case 4: return go<TX, TY, 4, VEC>(q, grad, s);
+        case 16: return go<TX, TY, 16, VEC>(q, grad, s);
+        case 64: return go<TX, TY, 64, VEC>(q, grad, s);
+        case 128: return go<TX, TY, 128, VEC>(q, grad, s);
+        case 256: return go<TX, TY, 256, VEC>(q, grad, s);
+        case 512: return go<TX, TY, 512, VEC>(q, grad, s);
+        default: return go<TX, TY, 1024, VEC>(q, grad, s);
     }
 }
 template <typename TX, typename TY> int by_vec(const Norm& q, bool grad, hipStream_t s) {
