@@ -21,6 +21,8 @@ namespace {
 constexpr int SHORT = 1024;                 // rows up to here stay in a wave's registers
 constexpr int SEGMENT = 4096;               // shortest part of a long row that is worth a workgroup of its own
 constexpr long ONE_WAVE = 2048;             // long rows from which on a wave takes one
+constexpr long SHARED_WAVE = 4096;          // short rows from which on several share a wave also beyond 256 entries (32768 x 361 f16: k 0 20 -> 10 us,
+                                            // k 20 95 -> 52; but 1024 x 361, k 20 8.4 -> 11.7: a wave's own chain is longer)
 
 struct Rows {
     const void* raw; long raw_stride;       // elements
@@ -94,7 +96,8 @@ template <int N> __device__ __forceinline__ float max_of(const float (&x)[N]) {
 
 // ---- short rows: G lanes hold a row, N entries each -----------------------------------------------------------------------------
 // Entry j of the row is with lane j % G.  Loads are coalesced whatever the rows' alignment; everything else is in registers, the
-// reductions are DPP.  What bounds it is instructions per row, not bytes, so up to 256 entries four rows share a wave.
+// reductions are DPP.  What bounds it is instructions per row, not bytes, so up to 256 entries four rows share a wave, and where there are many
+// rows four up to 512 and two up to 1024.
 template <typename T, int G, int N>
 __global__ void __launch_bounds__(256) logprobs_rows_kernel(Rows q) {
     const int gl = threadIdx.x & (G - 1);
@@ -493,6 +496,10 @@ template <typename T, typename Q> void pick_short(const Q& q, hipStream_t s) {
     else if (q.A <= 128) go_short<T, 16, 8>(q, s);
     else if (q.A <= 192) go_short<T, 16, 12>(q, s);
     else if (q.A <= 256) go_short<T, 16, 16>(q, s);
+    else if (q.A <= 384 && q.R >= SHARED_WAVE) go_short<T, 16, 24>(q, s);
+    else if (q.A <= 512 && q.R >= SHARED_WAVE) go_short<T, 16, 32>(q, s);
+    else if (q.A <= 768 && q.R >= SHARED_WAVE) go_short<T, 32, 24>(q, s);
+    else if (q.R >= SHARED_WAVE) go_short<T, 32, 32>(q, s);
     else if (q.A <= 512) go_short<T, 64, 8>(q, s);
     else go_short<T, 64, 16>(q, s);
 }

@@ -60,16 +60,18 @@ __device__ __forceinline__ unsigned lane_u(unsigned v, int lane) { return (unsig
 
 struct Sum { static __device__ __forceinline__ float f(float a, float b) { return a + b; } };
 struct Max { static __device__ __forceinline__ float f(float a, float b) { return fmaxf(a, b); } };
-// G = 4: a quad; G = 16: one DPP row; G = 64: the wave (row rotations, then the four rows' values through scalar registers)
+// G = 4: a quad; G = 16: one DPP row; G = 32: two, through a shuffle; G = 64: the wave (row rotations, then the four rows' values through scalar registers)
 template <int G, typename Op> __device__ __forceinline__ float reduce(float v) {
     if constexpr (G == 4) { v = Op::f(v, ror<0xb1>(v)); return Op::f(v, ror<0x4e>(v)); }
     v = Op::f(v, ror<0x128>(v)); v = Op::f(v, ror<0x124>(v)); v = Op::f(v, ror<0x122>(v)); v = Op::f(v, ror<0x121>(v));
+    if constexpr (G == 32) v = Op::f(v, __shfl_xor(v, 16));
     if constexpr (G == 64) v = Op::f(Op::f(lane_f(v, 0), lane_f(v, 16)), Op::f(lane_f(v, 32), lane_f(v, 48)));
     return v;
 }
 template <int G> __device__ __forceinline__ unsigned reduce_max_u(unsigned v) {
     v = max(v, (unsigned)ror<0x128>((int)v)); v = max(v, (unsigned)ror<0x124>((int)v));
     v = max(v, (unsigned)ror<0x122>((int)v)); v = max(v, (unsigned)ror<0x121>((int)v));
+    if constexpr (G == 32) v = max(v, (unsigned)__shfl_xor((int)v, 16));
     if constexpr (G == 64) v = max(max(lane_u(v, 0), lane_u(v, 16)), max(lane_u(v, 32), lane_u(v, 48)));
     return v;
 }

@@ -93,7 +93,8 @@ def check_logprobs(raw, actions, valid, k, out):
     return w
 
 
-LOGPROBS = [(1, 1), (3, 2), (5, 16), (6, 33), (70, 81), (9, 97), (4, 169), (3, 256), (5, 257), (4, 513), (3, 1024), (3, 1025), (2, 5003), (600, 4100), (2, 32768), (1, 131071)]
+LOGPROBS = [(1, 1), (3, 2), (5, 16), (6, 33), (70, 81), (9, 97), (4, 169), (3, 256), (5, 257), (4, 513), (3, 1024), (3, 1025), (2, 5003), (600, 4100), (2, 32768), (1, 131071),
+            (4099, 300), (4097, 512), (4098, 600), (4096, 1000), (2050, 1500)]
 
 
 @pytest.mark.gpu
