@@ -11,6 +11,7 @@
 // every time.  32768 x 512, f32 stream, f16 branches with gates: forward 42 us for 235 MB (5.5 TB/s), backward 68 us for 369 MB (5.4 TB/s) and
 // 4 us for the sums; 4096 x 771 f32 14 + 21 + 4 us; 8192 x 4096 bf16 forward 58 us for 335 MB (5.8 TB/s); a copy of 4 GiB runs at 4.75 TB/s, of 32 MiB at 6.6.
 #include "bl_train.h"
+#include "bl_host.h"
 
 #pragma clang fp contract(off)
 
@@ -160,28 +161,52 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(Norm q) {
     }
 }
 
+// A lane's sums over its rows, for dpost, dpre and a gate per channel.  In registers; at 16 waves per workgroup, where a lane has 128 of them
+// and needs 150, in LDS (its own places, no bank conflict): 2048 x 8192 f32 / f16 124 us with its launches, 196 with what spilled from registers;
+// 2048 x 8191, whose single elements need more addresses, 259 with some spills left (445)
+enum { POST, PRE, GATE };
+template <int G, int N> struct Columns {
+    float v[3][N];
+    __device__ __forceinline__ explicit Columns(float*) {
+#pragma unroll
+        for (int a = 0; a < 3; a++)
+#pragma unroll
+            for (int i = 0; i < N; i++) v[a][i] = 0.f;
+    }
+    __device__ __forceinline__ void add(int a, int i, float x, float y) { v[a][i] = fmaf(x, y, v[a][i]); }
+    __device__ __forceinline__ float get(int a, int i) const { return v[a][i]; }
+};
+template <int N> struct Columns<1024, N> {
+    float* v;
+    __device__ __forceinline__ explicit Columns(float* lds) : v(lds + threadIdx.x) {
+#pragma unroll
+        for (int i = 0; i < 3 * N; i++) v[1024 * i] = 0.f;
+    }
+    __device__ __forceinline__ void add(int a, int i, float x, float y) { v[1024 * (a * N + i)] = fmaf(x, y, v[1024 * (a * N + i)]); }
+    __device__ __forceinline__ float get(int a, int i) const { return v[1024 * (a * N + i)]; }
+};
+
 template <typename TX, typename TY, int G, int N, int VEC>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
+    extern __shared__ __align__(16) float wide[];
     __shared__ float lds[32];
     constexpr int T = G > 256 ? G : 256, ROWS = T / G;
     __shared__ float cols[ROWS > 1 ? 3 * N * G + 1 : 1];
     const int gl = threadIdx.x & (G - 1);
     int set = 0;
     float post[N], pre[N], gate[N];
-    constexpr bool KEEP = G < 1024;         // gains in registers for all rows; a workgroup of 16 waves has no room, and a row's are read with it
-    auto gains = [&] {
-        if (q.post) read<G, VEC>(q.post, gl, q.W, post);
-        if (q.gh) read<G, VEC>(q.pre, gl, q.W, pre);
-        if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
-    };
+    // gains and channel gates: in registers for all rows, or (16 waves) read again where a row needs them
+    constexpr bool KEEP = G < 1024;
+    auto read_post = [&] { if (q.post) read<G, VEC>(q.post, gl, q.W, post); };
+    auto read_pre = [&] { if (q.gh) read<G, VEC>(q.pre, gl, q.W, pre); };
+    auto read_gate = [&] { if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate); };
     if (!q.post)
 #pragma unroll
         for (int i = 0; i < N; i++) post[i] = 1.f;
-    if constexpr (KEEP) gains();
+    if constexpr (KEEP) { read_post(); read_pre(); read_gate(); }
     const float alpha = q.alpha ? *q.alpha : 1.f;
-    float spost[N], spre[N], sgate[N], salpha = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; i++) spost[i] = spre[i] = sgate[i] = 0.f;
+    Columns<G, N> sums(wide);
+    float salpha = 0.f;
     for (long r0 = (long)blockIdx.x * ROWS; r0 < q.R; r0 += (long)gridDim.x * ROWS) {
         const long row = r0 + group_of<G>(), at = row < q.R ? row : q.R - 1;
         const bool live = row < q.R;
@@ -193,7 +218,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
         if (q.kind == BL_GATE_FULL) eg.fetch((const TY*)q.gate + at * q.gs, gl, q.W);
         if (q.gx) ez.fetch((const TX*)q.gx + at * q.gxs, gl, q.W);
         if (q.gh) et.fetch((const TY*)q.gh + at * q.ghs, gl, q.W);
-        if constexpr (!KEEP) gains();
+        if constexpr (!KEEP) { read_post(); read_gate(); }
         // (beyond W everything is 0, so nothing there counts; the sigmoid is computed twice rather than held)
         float x[N], z[N], n[N];
         ex.get(x, gl, q.W);
@@ -219,10 +244,11 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
         if (q.gh) {
             float t[N], c = 0.f;
             et.get(t, gl, q.W);
+            if constexpr (!KEEP) read_pre();
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 x[i] *= rx;                                                          // xn
-                if (live) spre[i] = fmaf(t[i], x[i], spre[i]);
+                if (live) sums.add(PRE, i, t[i], x[i]);
                 t[i] *= pre[i];
                 c = fmaf(t[i], x[i], c);
             }
@@ -234,17 +260,18 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
         if (live) write<G, VEC>((TX*)q.dx + at * q.W, gl, q.W, z);
         if (!q.y) continue;
         float c = 0.f, cg = 0.f, dn[N];
+        if constexpr (!KEEP) { read_post(); read_gate(); }
         if (q.kind != BL_GATE_NONE) {
             float dg[N];
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const Gate g = sigmoid(gate[i]);
                 const float v = alpha * z[i], vn = v * n[i], sp = g.s * post[i];
-                if (live) { salpha = fmaf(z[i], n[i] * sp, salpha); spost[i] = fmaf(vn, g.s, spost[i]); }
+                if (live) { salpha = fmaf(z[i], n[i] * sp, salpha); sums.add(POST, i, vn, g.s); }
                 dn[i] = v * sp;
                 c = fmaf(dn[i], n[i], c);
                 dg[i] = vn * post[i] * g.ds;
-                if (live) sgate[i] += dg[i];
+                if (live && q.kind == BL_GATE_CHANNEL) sums.add(GATE, i, dg[i], 1.f);
                 cg += dg[i];
             }
             if (q.kind == BL_GATE_FULL && q.dgate && live) write<G, VEC>((TY*)q.dgate + at * q.dgs, gl, q.W, dg);
@@ -256,7 +283,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const float v = alpha * z[i];
-                if (live) { salpha = fmaf(z[i], n[i] * post[i], salpha); spost[i] = fmaf(v, n[i], spost[i]); }
+                if (live) { salpha = fmaf(z[i], n[i] * post[i], salpha); sums.add(POST, i, v, n[i]); }
                 dn[i] = v * post[i];
                 c = fmaf(dn[i], n[i], c);
             }
@@ -275,7 +302,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int j = column<G, VEC>(gl, i);
-            if (j < q.W) { out[j] = spost[i]; out[q.W + j] = spre[i]; out[2 * q.W + j] = sgate[i]; }
+            if (j < q.W) { out[j] = sums.get(POST, i); out[q.W + j] = sums.get(PRE, i); out[2 * q.W + j] = sums.get(GATE, i); }
         }
         if (gl == 0) out[3 * q.W] = salpha;
     } else {
@@ -285,9 +312,8 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_grad_kernel(Norm q) {
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     const int k = gl + G * i;
-                    cols[k] = g ? cols[k] + spost[i] : spost[i];
-                    cols[N * G + k] = g ? cols[N * G + k] + spre[i] : spre[i];
-                    cols[2 * N * G + k] = g ? cols[2 * N * G + k] + sgate[i] : sgate[i];
+#pragma unroll
+                    for (int a = 0; a < 3; a++) cols[a * N * G + k] = g ? cols[a * N * G + k] + sums.get(a, i) : sums.get(a, i);
                 }
                 if (gl == 0) cols[3 * N * G] = g ? cols[3 * N * G] + salpha : salpha;
             }
@@ -327,8 +353,7 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(Sums q) {
 // ---- host --------------------------------------------------------------------------------------------------------------------------
 // Lanes of a row, 8 elements each: the fewest that hold it -- 16 rows to a wave up to 32 wide, a row to a wave up to 512 (no barrier), to a
 // workgroup from 1025 on.  (16 elements per lane need 300 registers in the backward pass: 16384 x 768 f32 114 us with its launches, with 8 per lane in two
-// waves 84.)  Beyond 4096 wide sixteen waves leave a lane 128 registers of the 150 it needs, and what spills bounds the backward pass: 2048 x 8192 f32 / f16 196 us,
-// 1.9 TB/s, where 4096 x 4096 takes 98; the forward pass fits (44 us, 5.4 TB/s)
+// waves 84)
 constexpr int N = 8;
 int lanes_of(int W) { return W <= 32 ? 4 : W <= 128 ? 16 : W <= 512 ? 64 : W <= 1024 ? 128 : W <= 2048 ? 256 : W <= 4096 ? 512 : 1024; }
 // workgroups of the backward pass: each leaves 3 W + 1 sums, so no more than keep the chip full
@@ -341,8 +366,12 @@ bool aligned(const void* p, long stride, int size) { return !p || ((reinterpret_
 
 template <typename TX, typename TY, int G, int VEC> int go(const Norm& q, bool grad, hipStream_t s) {
     constexpr int T = G > 256 ? G : 256, ROWS = T / G;
-    if (grad) hipLaunchKernelGGL((norm_grad_kernel<TX, TY, G, N, VEC>), dim3((unsigned)blocks_of(q.R, q.W)), dim3(T), 0, s, q);
-    else {
+    if (grad) {
+        constexpr size_t bytes = G == 1024 ? 3 * N * G * sizeof(float) : 0;
+        static size_t raised[64];
+        if (!bl_raise_lds_limit((const void*)norm_grad_kernel<TX, TY, G, N, VEC>, bytes, raised)) return BL_ELAUNCH;
+        hipLaunchKernelGGL((norm_grad_kernel<TX, TY, G, N, VEC>), dim3((unsigned)blocks_of(q.R, q.W)), dim3(T), bytes, s, q);
+    } else {
         const long need = (q.R + ROWS - 1) / ROWS;
         hipLaunchKernelGGL((norm_kernel<TX, TY, G, N, VEC>), dim3((unsigned)(need < 2048 ? need : 2048)), dim3(T), 0, s, q);
     }
