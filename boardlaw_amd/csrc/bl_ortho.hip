@@ -4,7 +4,7 @@
 //
 // takes every singular value s to a s + b s^3 + c s^5 and again, i.e. towards 1.  The iteration multiplies what is small by up to 3.4 a
 // step: with f16 or bf16 operands the rounding of the large directions drowns the small ones of a low-rank gradient (3.7 % / 30 % of the
-// result on rank 8 + 1 % noise).  So every operand is a pair of f16 numbers hi + lo (22 bits and lo's sign), a product is hi hi + hi lo +
+// result on rank 8 + 1 % noise).  So every operand (beyond few rows, below) is a pair of f16 numbers hi + lo (22 bits and lo's sign), a product is hi hi + hi lo +
 // lo hi on v_mfma_f32_32x32x16_f16 with f32 sums (the dropped lo lo is 2^-24 of the product: what f32 rounding costs), 3/16 of the matrix
 // rate instead of the f32 MFMA's 1/16.  Operands carry a factor 2^13: entries of X and B stay below 3 (the quintic maps [0, 1.21] into
 // itself), so hi < 2^15, and lo keeps its bits above f16's smallest steps down to entries of 2^-14.
@@ -392,10 +392,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
     }
 }
 
-// ---- m <= 64 and n <= 64 NB: one workgroup takes a matrix through all of it in LDS ------------------------------------------------------
+// ---- 32 < m <= 64 and n <= 64 NB <= 128: one workgroup takes a matrix through all of it in LDS ------------------------------------------------
 // 15 dependent products of a few hundred cycles each: launches (3 to 5 us apiece) would be nearly all of the time.  Here products cost next
 // to nothing, so operands are three f16 numbers (33 bits) and a product six: a small matrix is often nearly singular, and sums this
-// short leave f32 so little error of their own that 22 bits would show (8 x 8: up to 4.8 times f32's).
+// short leave f32 so little error of their own that 22 bits would show.
 constexpr int TRIPLE = 3 * FRAG;
 __device__ __forceinline__ int triple_at(int rb, int kb, int KB) { return (rb * KB + kb) * TRIPLE; }
 __device__ __forceinline__ void split(float v, f16 (&o)[3]) {
@@ -530,12 +530,187 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
     }
 }
 
+// ---- few rows: the iteration on the m x m side, in f64 --------------------------------------------------------------------------------
+// Every X of the iteration is Q G with Q a polynomial of G G^T, so that with A = X X^T the steps are  P = a I + b A + c A^2,  Q = P Q,  A = P A P
+// and G comes in twice: for its Gram matrix and for Q G.  Sums over few rows leave f32 so little error of its own that operands of 22 bits would
+// show (against the f32 form's: 8 x 129 2.7 times, 2 x 500 likewise, 32 x 200 1.55, 64 x 300 1.04), and 33 bits with f32 sums still do (8 x 8 1.75).  m x m
+// products on v_mfma_f64_16x16x4_f64 are few, and what is left is the result's own rounding.  A column's sums over k may be taken
+// in any order, so a lane loads 4 consecutive k; one fragment is both operands of a Gram product.
+// Where it is used: up to 32 rows at any width, up to 64 beyond 128 wide.  us, beside the kernels above: 4 x 16 x 16 10.9 (19.2), 4 x 32 x 32 18.3 (21.2),
+// 4 x 8 x 400 15 (90), 4 x 32 x 200 27 (84), 4 x 64 x 300 85 (88), 64 x 1000 86 (102), 64 x 16384 133 (515); but 4 x 48 x 48 38 (23), 4 x 64 x 64 69 (25), 4 x 64 x 128 78 (41),
+// where three f16 numbers are as exact as f32.  The steps' f64 products bound it: 69 of 85 us at 64 x 300.
+typedef double d4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ d4 mfma(double x, double y, d4 acc) { return __builtin_amdgcn_mfma_f64_16x16x4f64(x, y, acc, 0, 0, 0); }
+// rows of 16 MT doubles, an odd number of 16s apart: the four rows that a fragment's lanes read lie in different banks
+constexpr int ONE_PART = 256, MOST_PARTS = 32;
+template <int MT> struct Few { static constexpr int MP = 16 * MT, LD = MP | 16, TILES = MT * (MT + 1) / 2, SIZE = MP * LD; };
+// tile t of those on and above the diagonal, column by column
+__device__ __forceinline__ void tile_at(int t, int& a, int& b) { b = 0; while (t > b) t -= ++b; a = t; }
+// a lane's 4 values of tile (a, b) of a product: row l / 16 + 4 i, column l % 16
+template <int LD> __device__ __forceinline__ int few_at(int a, int b, int i) { return (16 * a + (threadIdx.x >> 4 & 3) + 4 * i) * LD + 16 * b + (threadIdx.x & 15); }
+template <int LD> __device__ __forceinline__ int few_mirror(int a, int b, int i) { return (16 * b + (threadIdx.x & 15)) * LD + 16 * a + (threadIdx.x >> 4 & 3) + 4 * i; }
+
+// Gram matrix of columns c0 .. c1 - 1 of G into `to`: the waves take 16 columns in turn and are added in their order
+template <typename T, int MT> __device__ __forceinline__ void gram_few(const T* g, int m, int n, int tall, int c0, int c1, double* to) {
+    using F = Few<MT>;
+    const int wave = threadIdx.x >> 6, i = threadIdx.x & 15, h = threadIdx.x >> 4 & 3;
+    d4 acc[F::TILES] = {};
+    for (int k = c0 + 16 * wave; k < c1; k += 64) {
+        T raw[MT][4];
+#pragma unroll
+        for (int r = 0; r < MT; r++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int row = min(16 * r + i, m - 1), col = min(k + 4 * h + c, c1 - 1);
+                raw[r][c] = g[tall ? (long)col * m + row : (long)row * n + col];
+            }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            double x[MT];
+#pragma unroll
+            for (int r = 0; r < MT; r++) x[r] = 16 * r + i < m && k + 4 * h + c < c1 ? (double)(float)raw[r][c] : 0.;
+#pragma unroll
+            for (int b = 0, t = 0; b < MT; b++)
+#pragma unroll
+                for (int a = 0; a <= b; a++, t++) acc[t] = mfma(x[a], x[b], acc[t]);
+        }
+    }
+    for (int w = 0; w < 4; w++) {
+        if (wave == w) {
+#pragma unroll
+            for (int b = 0, t = 0; b < MT; b++)
+#pragma unroll
+                for (int a = 0; a <= b; a++, t++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int at = few_at<F::LD>(a, b, j);
+                        const double v = w ? to[at] + acc[t][j] : acc[t][j];
+                        to[at] = v;
+                        if (w == 3 && a != b) to[few_mirror<F::LD>(a, b, j)] = v;
+                    }
+        }
+        __syncthreads();
+    }
+}
+// a part of the columns per workgroup; whole matrices of MP x MP, added up by few_rows_kernel
+template <typename T, int MT> __global__ void __launch_bounds__(256) few_gram_kernel(Mats q, int m, int n, int tall, double* parts) {
+    extern __shared__ __align__(16) char smem[];
+    using F = Few<MT>;
+    double* A = (double*)smem;
+    gram_few<T, MT>((const T*)q.in[blockIdx.y], m, n, tall, (int)((long)n * blockIdx.x / gridDim.x), (int)((long)n * (blockIdx.x + 1) / gridDim.x), A);
+    double* to = parts + ((long)blockIdx.y * gridDim.x + blockIdx.x) * F::MP * F::MP;
+    for (int e = threadIdx.x; e < F::MP * F::MP; e += 256) to[e] = A[e / F::MP * F::LD + e % F::MP];
+}
+
+// S = 0: one workgroup takes a matrix through all of it.  Otherwise from the Gram matrix's S parts, each of a matrix's workgroups through the (same)
+// steps and then its own columns of Q G: that costs what a launch of its own for the steps would, without the launch
+template <typename T, int MT>
+__global__ void __launch_bounds__(256) few_rows_kernel(Mats q, int m, int n, int tall, int steps, float eps, const double* parts, int S) {
+    extern __shared__ __align__(16) char smem[];
+    using F = Few<MT>;
+    constexpr int MP = F::MP, LD = F::LD, EACH = (F::TILES + 3) / 4;
+    double *A = (double*)smem, *P = A + F::SIZE, *Q = P + F::SIZE;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, h = lane >> 4;
+    const T* g = (const T*)q.in[blockIdx.y];
+    if (S == 0) gram_few<T, MT>(g, m, n, tall, 0, n, A);
+    else {
+        for (int e = threadIdx.x; e < MP * MP; e += 256) {
+            const double* from = parts + (long)blockIdx.y * S * MP * MP + e;
+            double v = 0.;
+#pragma unroll 4
+            for (int s = 0; s < S; s++) v += from[(long)s * MP * MP];
+            A[e / MP * LD + e % MP] = v;
+        }
+        __syncthreads();
+    }
+    double trace = lane < MP ? A[lane * LD + lane] : 0.;        // |G|^2: neither 2^100 nor 2^-100 as a loss scale overflows or vanishes
+    for (int o = 32; o; o >>= 1) trace += __shfl_xor(trace, o);
+    const double inv = 1. / (sqrt(trace) + (double)eps);
+    __syncthreads();
+    for (int e = threadIdx.x; e < F::SIZE; e += 256) A[e] *= inv * inv;        // (what lies between the rows is nobody's)
+    __syncthreads();
+    // a product of two symmetric matrices that commute, which is symmetric: its tiles on and above the diagonal, dealt out to the waves
+    auto product = [&](const double* x, const double* y, d4 (&acc)[EACH]) {
+        int a[EACH], b[EACH];
+#pragma unroll
+        for (int u = 0; u < EACH; u++) { tile_at(min(wave + 4 * u, F::TILES - 1), a[u], b[u]); acc[u] = d4{}; }
+#pragma unroll
+        for (int k = 0; k < MP; k += 4)
+#pragma unroll
+            for (int u = 0; u < EACH; u++) acc[u] = mfma(x[(k + h) * LD + 16 * a[u] + i], y[(k + h) * LD + 16 * b[u] + i], acc[u]);
+    };
+    auto put = [&](double* to, auto value) {                 // value(place, i-th of tile u)
+#pragma unroll
+        for (int u = 0; u < EACH; u++) {
+            int a, b;
+            tile_at(wave + 4 * u, a, b);
+            if (wave + 4 * u < F::TILES)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int at = few_at<LD>(a, b, j);
+                    const double v = value(at, u, j);
+                    to[at] = v;
+                    if (a != b) to[few_mirror<LD>(a, b, j)] = v;
+                }
+        }
+    };
+    for (int it = 0; it < steps; it++) {
+        const bool last = it + 1 == steps;
+        d4 r[EACH], s[EACH];
+        product(A, A, r);
+        put(P, [&](int at, int u, int j) { return (at / LD == at % LD ? 3.4445 : 0.) + (-4.7750 * A[at] + 2.0315 * r[u][j]); });
+        __syncthreads();
+        if (it) product(P, Q, r);
+        if (!last) product(P, A, s);
+        __syncthreads();
+        put(Q, [&](int at, int u, int j) { return it ? r[u][j] : inv * P[at]; });
+        if (!last) put(A, [&](int, int u, int j) { return s[u][j]; });
+        __syncthreads();
+        if (last) break;
+        product(P, A, s);
+        __syncthreads();
+        put(A, [&](int, int u, int j) { return s[u][j]; });
+        __syncthreads();
+    }
+    // Q G, 16 columns of a wave at a time, read before they are written.  A tall G is its transpose here, and so is its tile
+    T* out = (T*)q.out[blockIdx.y];
+    for (int c0 = (blockIdx.x * 4 + wave) * 16; c0 < n; c0 += gridDim.x * 64) {
+        T raw[MP / 4];
+        double x[MP / 4];
+#pragma unroll
+        for (int k = 0; k < MP / 4; k++) {
+            const int row = min(4 * k + h, m - 1), col = min(c0 + i, n - 1);
+            raw[k] = g[tall ? (long)col * m + row : (long)row * n + col];
+        }
+#pragma unroll
+        for (int k = 0; k < MP / 4; k++) x[k] = 4 * k + h < m && c0 + i < n ? (double)(float)raw[k] : 0.;
+#pragma unroll
+        for (int a = 0; a < MT; a++) {
+            d4 acc = {};
+#pragma unroll
+            for (int k = 0; k < MP / 4; k++) {
+                const double y = Q[(4 * k + h) * LD + 16 * a + i];
+                acc = tall ? mfma(x[k], y, acc) : mfma(y, x[k], acc);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int row = 16 * a + (tall ? i : h + 4 * j), col = c0 + (tall ? h + 4 * j : i);
+                if (row < m && col < n) out[tall ? (long)col * m + row : (long)row * n + col] = (T)(float)acc[j];
+            }
+        }
+    }
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------------------------
 struct Plan { long x, a, norm; long total(int count) const { return count * (3 * x + 2 * a) * (long)sizeof(f16) + norm; } };
 Plan plan_of(int m, int n) {                // halves of one matrix: X (and each X^T), A (and B); bytes of the norms' parts
     const long mp = up(m), np = up(n);
     return {2 * mp * np, 2 * mp * mp, MANY * PARTS * (long)sizeof(double)};
 }
+bool few_rows(int m, int n) { return m <= 32 || (m <= 64 && n > 128); }
+// parts of a Gram matrix, by the columns alone (a matrix's result does not depend on its batch)
+int few_parts(int n) { return n <= ONE_PART ? 0 : (n + ONE_PART - 1) / ONE_PART < MOST_PARTS ? (n + ONE_PART - 1) / ONE_PART : MOST_PARTS; }
+long few_bytes(int count, int m, int n) { const long mp = (m + 15) / 16 * 16, s = few_parts(n); return count * (s > 0 ? s : 1) * mp * mp * (long)sizeof(double); }
 template <int MODE, int F> bool wide(const Product& p, const Mats& q, hipStream_t s) {
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     constexpr size_t bytes = 4 * (F + 2) * 4096;
@@ -562,15 +737,28 @@ template <typename T, int NB> bool small(const Product& p, const Mats& q, int st
     hipLaunchKernelGGL((ortho_small_kernel<T, NB>), dim3(p.count), dim3(256), bytes, s, q, p, steps, eps);
     return true;
 }
+template <typename T, int MT> int few(const Mats& q, int c, int m, int n, int tall, int steps, float eps, double* parts, hipStream_t s) {
+    using F = Few<MT>;
+    constexpr size_t one = F::SIZE * sizeof(double);
+    static size_t raised[64];
+    if (!bl_raise_lds_limit((const void*)few_rows_kernel<T, MT>, 3 * one, raised)) return BL_ELAUNCH;
+    const int S = few_parts(n), most = (n + 63) / 64, want = 256 / c;
+    if (S) hipLaunchKernelGGL((few_gram_kernel<T, MT>), dim3(S, c), dim3(256), one, s, q, m, n, tall, parts);
+    hipLaunchKernelGGL((few_rows_kernel<T, MT>), dim3(S == 0 ? 1 : want < most ? want : most, c), dim3(256), 3 * one, s, q, m, n, tall, steps, eps, parts, S);
+    return check_launch();
+}
 template <typename T> int run(const Mats& q, int c, int m, int n, int tall, int dtype, int steps, float eps, const Plan& plan, void* workspace, hipStream_t s) {
     const int mp = up(m), np = up(n);
+    double* parts = (double*)workspace;
+    if (few_rows(m, n))
+        return m <= 16 ? few<T, 1>(q, c, m, n, tall, steps, eps, parts, s) : m <= 32 ? few<T, 2>(q, c, m, n, tall, steps, eps, parts, s)
+             : m <= 48 ? few<T, 3>(q, c, m, n, tall, steps, eps, parts, s) : few<T, 4>(q, c, m, n, tall, steps, eps, parts, s);
     if (m <= 64 && n <= 128) {
         Product p{};
         p.m = m; p.n = n; p.tall = tall; p.dtype = dtype; p.count = c;
         if (!(n <= 64 ? small<T, 1>(p, q, steps, eps, s) : small<T, 2>(p, q, steps, eps, s))) return BL_ELAUNCH;
         return check_launch();
     }
-    double* parts = (double*)workspace;
     f16* X = (f16*)((char*)workspace + plan.norm);
     f16* XT[2] = {X + c * plan.x, X + 2 * c * plan.x};
     f16* A = X + 3 * c * plan.x;
@@ -597,7 +785,8 @@ extern "C" {
 long bl_orthogonalize_workspace(int count, int rows, int cols) {
     if (count <= 0 || rows <= 0 || cols <= 0 || rows > BL_ORTHO_MAX || cols > BL_ORTHO_MAX) return 0;
     const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-    return plan_of(m, n).total(count < MANY ? count : MANY);
+    if (count > MANY) count = MANY;
+    return few_rows(m, n) ? few_bytes(count, m, n) : plan_of(m, n).total(count);
 }
 
 int bl_orthogonalize(const void* const* host_in, void* const* host_out, int count, int dtype, int rows, int cols, int steps, float eps,

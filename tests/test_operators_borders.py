@@ -1,0 +1,73 @@
+"""The learner-step operators where they could go wrong without the tests of test_operators.py showing it: precision against the f32 form's, values at the
+types' borders, ways of calling that autograd, tracing and views allow, and rows enough for every loop."""
+import math
+
+import pytest
+import torch
+
+from test_operators import U, half_step
+
+
+# ------------------------------------------------------------------------------------------------------------ orthogonalize
+
+def iteration(g, dtype, steps=5, eps=1e-7):
+    """The Newton-Schulz iteration in elementary products of one type, on the side with fewer rows."""
+    tall = g.shape[0] > g.shape[1]
+    x = (g.T if tall else g).to(dtype)
+    x = x / (x.double().square().sum().sqrt() + eps).to(dtype)
+    for _ in range(steps):
+        a = x @ x.T
+        x = 3.4445 * x + (-4.7750 * a + 2.0315 * (a @ a)) @ x
+    return x.T if tall else x
+
+
+def gradient_like(m, n, kind, seed):
+    """randn: all singular values alike; decay: falling like a Linear's gradient; rank8: eight directions and 1 % noise; steep: down to a thousandth."""
+    gen = torch.Generator('cuda').manual_seed(seed)
+    normal = lambda *s: torch.randn(s, generator=gen, device='cuda', dtype=torch.float64)
+    q = min(m, n)
+    if kind == 'randn':
+        return normal(m, n)
+    if kind == 'decay':
+        return .01 * (normal(m, q) * torch.arange(1, q + 1, device='cuda').double().rsqrt()) @ normal(q, n) / q
+    if kind == 'rank8':
+        return normal(m, 8) @ normal(8, n) + .01 * normal(m, n)
+    u, v = torch.linalg.qr(normal(m, q))[0], torch.linalg.qr(normal(n, q))[0]
+    return (u * torch.logspace(-3, 0, q, device='cuda', dtype=torch.float64)) @ v.T
+
+
+KINDS = ['randn', 'decay', 'rank8', 'steep']
+FEW = [(1, 1), (1, 700), (2, 500), (8, 8), (8, 129), (129, 8), (8, 4000), (16, 16), (16, 162), (17, 256), (17, 257), (32, 200), (200, 32), (33, 300), (48, 129), (64, 200), (63, 1001),
+       (1001, 63), (3, 16384), (5000, 40)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('m,n', FEW)
+def test_few_rows_are_exact_but_for_the_last_rounding(m, n, dtype):
+    """Up to 32 rows (columns), or 64 beside more than 128, are computed in f64: an entry is off by its rounding, through f32, and by what f64 leaves.  A Gram matrix is a random
+    walk of n + 20 m roundings off; the steps' product takes a deviation of A to at most 5e4 times that of the result (the derivative of the five steps'
+    polynomial, 1.5e7 at 0 and falling, times the square root of the eigenvalue); four deviations of the walk."""
+    from boardlaw_amd import optim
+    mats = [gradient_like(m, n, kind, m + n).to(dtype) for kind in KINDS]
+    for kind, g, o in zip(KINDS, mats, optim.orthogonalize(mats)):
+        want = iteration(g, torch.float64)
+        tol = (half_step(dtype) + U) * want.abs() + 5e4 * 4 * (n + m + 20 * min(m, n)) ** .5 * 2. ** -53 + torch.finfo(dtype).tiny * half_step(dtype) * 2
+        off = (o.double() - want).abs() / tol
+        assert o.dtype == dtype and off.max() <= 1, (kind, float(off.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('count,m,n', [(3, 20, 24), (3, 20, 700), (40, 600, 20), (3, 64, 1000), (3, 50, 60), (3, 100, 150), (35, 130, 140)])
+def test_orthogonalize_in_place(count, m, n):
+    """The C entry point may write over its input; more matrices than one launch takes, each its own."""
+    import ctypes
+    from boardlaw_amd import _native, optim
+    L = _native.lib()
+    mats = [gradient_like(m, n, KINDS[i % 4], i).float() for i in range(count)]
+    want = [optim.orthogonalize(g) for g in mats]
+    assert all(torch.equal(a, b) for a, b in zip(optim.orthogonalize(mats), want))
+    work = torch.empty(L.bl_orthogonalize_workspace(count, m, n), dtype=torch.uint8, device='cuda')
+    at = (ctypes.c_void_p * count)(*[g.data_ptr() for g in mats])
+    _native.check(L.bl_orthogonalize(at, at, count, 0, m, n, 5, 1e-7, work.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    assert all(torch.equal(a, b) for a, b in zip(mats, want))
