@@ -41,6 +41,9 @@ __device__ __forceinline__ long frag_at(int rb, int kb, int KB) { return ((long)
 
 __device__ __forceinline__ void split(float v, f16& hi, f16& lo) { hi = (f16)v; lo = (f16)(v - (float)hi); }
 
+// 1 / (|G| + eps); 0 for a zero matrix without an eps, whose result is zeros too
+__device__ __forceinline__ double reciprocal(double square, float eps) { const double d = sqrt(square) + (double)eps; return d == 0. ? 0. : 1. / d; }
+
 // ---- |G|^2 in parts, in f64: neither 2^100 nor 2^-100 as a loss scale overflows or vanishes ----
 template <typename T> __global__ void __launch_bounds__(256) norm_parts_kernel(Mats q, long total, double* parts) {
     __shared__ double lds[4];
@@ -70,7 +73,7 @@ __global__ void __launch_bounds__(256) lay_out_kernel(Mats q, int m, int n, int 
     const T* g = (const T*)q.in[blockIdx.z];
     double ss = parts[blockIdx.z * PARTS + (threadIdx.x & 63)];
     for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
-    const double inv = (double)SCALE / (sqrt(ss) + (double)eps);
+    const double inv = (double)SCALE * reciprocal(ss, eps);
     const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
     for (int e = threadIdx.x; e < 1024; e += 256) {
         const int i = e >> 5, j = e & 31;                       // i: the slow index of G
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
     for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
     if (lane == 0) sums[wave] = ss;
     __syncthreads();
-    const double inv = (double)SCALE / (sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + (double)eps);
+    const double inv = (double)SCALE * reciprocal((sums[0] + sums[1]) + (sums[2] + sums[3]), eps);
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
         const int e = threadIdx.x + 256 * i, r = p.tall ? e % 64 : e / NP, col = p.tall ? e / 64 : e % NP;
@@ -625,7 +628,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(Mats q, int m, int n, int
     }
     double trace = lane < MP ? A[lane * LD + lane] : 0.;        // |G|^2: neither 2^100 nor 2^-100 as a loss scale overflows or vanishes
     for (int o = 32; o; o >>= 1) trace += __shfl_xor(trace, o);
-    const double inv = 1. / (sqrt(trace) + (double)eps);
+    const double inv = reciprocal(trace, eps);
     __syncthreads();
     for (int e = threadIdx.x; e < F::SIZE; e += 256) A[e] *= inv * inv;        // (what lies between the rows is nobody's)
     __syncthreads();

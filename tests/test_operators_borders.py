@@ -71,3 +71,19 @@ def test_orthogonalize_in_place(count, m, n):
     at = (ctypes.c_void_p * count)(*[g.data_ptr() for g in mats])
     _native.check(L.bl_orthogonalize(at, at, count, 0, m, n, 5, 1e-7, work.data_ptr(), torch.cuda.current_stream().cuda_stream))
     assert all(torch.equal(a, b) for a, b in zip(mats, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('m,n', [(1, 1), (20, 24), (700, 20), (50, 60), (50, 100), (100, 150), (512, 512)])
+def test_orthogonalize_of_nothing(m, n):
+    """A zero matrix gives zeros with any eps, none among them, beside others; NaN and infinities take their own matrix only."""
+    from boardlaw_amd import optim
+    one = gradient_like(m, n, 'randn', 1).float()
+    nan, inf = one.clone(), one.clone()
+    nan[m // 2, n // 2], inf[-1, -1] = math.nan, math.inf
+    for eps in (0., 1e-7, 1e-45):
+        for dtype in (torch.float32, torch.float16, torch.bfloat16):
+            z, a, b, c = optim.orthogonalize([t.to(dtype) for t in (torch.zeros_like(one), one, nan, inf)], eps=eps)
+            assert (z == 0).all() and b.isnan().all() and c.isnan().all()
+            want = iteration(one.to(dtype), torch.float64, eps=eps)
+            assert (a.double() - want).norm() <= (half_step(dtype) + 2e-5) * want.norm()        # (the value itself: tested elsewhere)
