@@ -6,9 +6,12 @@
 // 32768 rows of 81), most of it in the engine's thread waiting for the interpreter.  Built by boardlaw_amd/build.py with the host compiler
 // against torch's headers; like libbl_torchgen.so it is tied to the torch it was built with.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -43,6 +46,19 @@ void device_check(const Tensor& first, std::initializer_list<const Maybe*> other
     }
 }
 
+// These operators are not torch's, so a tracer (torch.jit.trace, make_fx) would write down their empty outputs and not the call, and a
+// forward-mode tangent would be dropped: both without a word, unless refused
+bool traced() {
+    return at::tracer::impl::is_dispatch_enabled() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+}
+void refuse(const std::string& what) { raise(PyExc_NotImplementedError, what); }
+void transform_check(const char* name, std::initializer_list<const Maybe*> tensors) {
+    if (traced()) refuse(say(name, " cannot be traced: its kernels are not torch's, and the trace would hold their empty outputs"));
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Maybe* t : tensors)
+        if (*t && (*t)->_fw_grad(0).defined()) refuse(say(name, " has no forward-mode derivative: got a tensor with a tangent"));
+}
+
 void check(int rc) { TORCH_CHECK(rc == BL_OK, "libboardlaw_amd: ", bl_strerror(rc), " (code ", rc, ")"); }
 
 bl_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
@@ -60,7 +76,10 @@ Tensor rows_of(const Tensor& t, int64_t width) {
 Tensor solid(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 std::vector<int64_t> with_last(at::IntArrayRef lead, int64_t n) { std::vector<int64_t> s(lead.begin(), lead.end()); s.push_back(n); return s; }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
-void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "this operator is differentiable once: its backward pass does not run under create_graph=True"); }
+void once() {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "this operator is differentiable once: its backward pass does not run under create_graph=True");
+    TORCH_CHECK_NOT_IMPLEMENTED(!traced(), "this operator's backward pass cannot be traced");
+}
 
 // ---- log probabilities ----
 struct LogProbs { Tensor logp, entropy, top, top_logp, stats; };
@@ -118,6 +137,8 @@ py::tuple py_logprobs(const Tensor& raw, const Maybe& actions, const Maybe& vali
     type_check(code_of(raw.scalar_type()) >= 0, "raw must be float32, float16 or bfloat16, got ", raw.scalar_type());
     value_check(raw.dim() >= 1 && raw.size(-1) >= 1, "raw must be (..., A) with at least one move, got ", shape_of(raw.sizes()));
     value_check(k >= 0 && k <= BL_TOP_MAX, "k must be in 0 .. ", BL_TOP_MAX, ", got ", k);
+    const Maybe raw_ = raw;
+    transform_check("logprobs", {&raw_, &actions, &valid});
     device_check(raw, {&actions, &valid});
     const auto lead = raw.sizes().slice(0, raw.dim() - 1);
     const int64_t A = raw.size(-1);
@@ -218,6 +239,8 @@ py::tuple py_norm_residual(const Tensor& x, const Maybe& y, const Maybe& alpha, 
                            const std::optional<at::ScalarType>& dtype) {
     type_check(code_of(x.scalar_type()) >= 0, "x must be float32, float16 or bfloat16, got ", x.scalar_type());
     value_check(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= BL_NORM_MAX, "x must be (..., W) with W in 1 .. ", BL_NORM_MAX, ", got ", shape_of(x.sizes()));
+    const Maybe x_ = x;
+    transform_check("norm_residual", {&x_, &y, &alpha, &post, &gate, &pre});
     device_check(x, {&y, &alpha, &post, &gate, &pre});
     const auto lead = x.sizes().slice(0, x.dim() - 1);
     const int64_t W = x.size(-1);
@@ -269,6 +292,8 @@ std::vector<Tensor> py_orthogonalize(const std::vector<Tensor>& mats, int64_t st
         type_check(code_of(m.scalar_type()) >= 0, "matrices must be float32, float16 or bfloat16, got ", m.scalar_type());
         value_check(m.dim() == 2, "matrices must be two-dimensional, got ", shape_of(m.sizes()));
         value_check(m.size(0) <= BL_ORTHO_MAX && m.size(1) <= BL_ORTHO_MAX, "sides up to ", BL_ORTHO_MAX, " are supported, got ", shape_of(m.sizes()));
+        const Maybe m_ = m;
+        transform_check("orthogonalize", {&m_});
         device_check(m, {});
     }
     for (size_t i = 0; i < mats.size(); i++) {

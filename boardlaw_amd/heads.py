@@ -59,7 +59,7 @@ def logprobs(raw, actions=None, valid=None, k=0):
     -> arrdict of f32 `logp` (...) (with actions), `entropy` (...), `top` (..., k) int64 and `top_logp` (..., k) (with k).  The alternatives come
     in descending order, equal ones by index; where fewer than k moves are valid the rest is -1 and -inf.  An invalid given move
     has logp -inf, a missing one (-1) 0, one beyond the row NaN.  A row with no valid move has entropy 0.  Differentiable (once) in `raw` through
-    logp, entropy and top_logp; an invalid move's gradient is 0.  On the GPU only (bl_logprobs)."""
+    logp, entropy and top_logp; an invalid move's gradient is 0.  Neither forward-mode derivatives nor tracing.  On the GPU only (bl_logprobs)."""
     logp, entropy, best, best_logp = _native.ops().logprobs(raw, actions, valid, k)
     out = arrdict.arrdict()
     if logp is not None:

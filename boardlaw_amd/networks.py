@@ -34,7 +34,8 @@ def norm_residual(x, y=None, alpha=None, post=None, gate=None, pre=None, eps=1e-
         gate   what goes through the sigmoid: (..., W) or (..., 1) of y's type, or (W,) f32, one per channel (for a one-dimensional x: of the channel)
         dtype  h's type where y is None (default: x's); else it is y's
 
-    -> (x_out, h).  Computed in f32, each result rounded once; differentiable (once) in every tensor.  On the GPU only (bl_norm_residual)."""
+    -> (x_out, h).  Computed in f32, each result rounded once; differentiable (once) in every tensor, in reverse mode; not traced.
+    On the GPU only (bl_norm_residual)."""
     return _native.ops().norm_residual(x, y, alpha, post, gate, pre, eps, dtype)
 
 

@@ -87,3 +87,51 @@ def test_orthogonalize_of_nothing(m, n):
             assert (z == 0).all() and b.isnan().all() and c.isnan().all()
             want = iteration(one.to(dtype), torch.float64, eps=eps)
             assert (a.double() - want).norm() <= (half_step(dtype) + 2e-5) * want.norm()        # (the value itself: tested elsewhere)
+
+
+# ------------------------------------------------------------------------------------------------- ways of calling
+
+def calls(device):
+    """Each operator as a function of one tensor."""
+    from boardlaw_amd import heads, networks, optim
+    w = torch.ones(4, device=device)
+    base = torch.ones((3, 4), device=device)
+    return dict(logprobs=lambda t: heads.logprobs(t, k=2).entropy, stream=lambda t: networks.norm_residual(t, base, None, w, pre=w)[1],
+                branch=lambda t: networks.norm_residual(base, t, None, w, pre=w)[0], gate=lambda t: networks.norm_residual(base, base, gate=t)[0],
+                norm=lambda t: networks.norm_residual(t, pre=w)[1], orthogonalize=lambda t: optim.orthogonalize([t])[0])
+
+
+@pytest.mark.parametrize('name', ['logprobs', 'stream', 'branch', 'gate', 'norm', 'orthogonalize'])
+@pytest.mark.parametrize('device', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+def test_what_would_be_lost_is_refused(name, device):
+    """A tangent (also of a tensor that requires no gradient) and a tracer's call raise: the operators know neither.  Refused before the device is looked at."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f = calls(device)[name]
+    x = torch.randn((3, 4), device=device)
+    with forward_ad.dual_level():
+        for leaf in (x, x.clone().requires_grad_()):
+            dual = forward_ad.make_dual(leaf, torch.ones_like(x))
+            with pytest.raises(NotImplementedError, match='tangent'):
+                f(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match='tangent'):
+                f(dual)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(f, (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(f)(x[None].expand(2, 3, 4))
+    with pytest.raises(NotImplementedError, match='traced'):
+        torch.jit.trace(f, (x,), check_trace=False)
+    with pytest.raises(NotImplementedError, match='traced'):
+        make_fx(f)(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', ['logprobs', 'stream', 'branch', 'gate', 'norm'])
+def test_a_backward_pass_is_not_traced(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn((3, 4), device='cuda', requires_grad=True)
+    out = calls('cuda')[name](x)
+    with pytest.raises(NotImplementedError, match='traced'):
+        make_fx(lambda g: torch.autograd.grad(out, x, g, retain_graph=True))(torch.ones_like(out))
+    torch.autograd.grad(out, x, torch.ones_like(out))
