@@ -67,13 +67,15 @@ template <typename T = void> T* ptr(const Tensor& t) { return t.defined() ? stat
 long row_stride(const Tensor& t) { return t.defined() ? t.stride(0) : 0; }
 Tensor value(const Maybe& t) { return t ? *t : Tensor(); }
 
+// values as they lie in memory: a tensor whose sign is a flag (the imaginary part of a conjugated tensor) is written out
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // (..., width) as (rows, width) with a contiguous last dimension: a view where the layout allows one
 Tensor rows_of(const Tensor& t, int64_t width) {
     if (!t.defined()) return t;
-    const Tensor flat = t.dim() == 2 ? t : t.reshape({t.numel() / std::max<int64_t>(width, 1), width});
+    const Tensor p = plain(t), flat = p.dim() == 2 ? p : p.reshape({p.numel() / std::max<int64_t>(width, 1), width});
     return width == 1 || flat.stride(1) == 1 ? flat : flat.contiguous();
 }
-Tensor solid(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor solid(const Tensor& t) { return t.defined() ? plain(t).contiguous() : t; }
 std::vector<int64_t> with_last(at::IntArrayRef lead, int64_t n) { std::vector<int64_t> s(lead.begin(), lead.end()); s.push_back(n); return s; }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 void once() {
@@ -148,7 +150,7 @@ py::tuple py_logprobs(const Tensor& raw, const Maybe& actions, const Maybe& vali
     if (actions) {
         value_check(actions->sizes() == lead, "actions must be ", shape_of(lead), ", got ", shape_of(actions->sizes()));
         type_check(at::isIntegralType(actions->scalar_type(), false), "actions must be whole numbers, got ", actions->scalar_type());
-        a = actions->to(at::kLong).reshape(-1).contiguous();
+        a = solid(actions->to(at::kLong).reshape(-1));
     }
     if (valid) {
         type_check(valid->scalar_type() == at::kBool, "valid must be bool, got ", valid->scalar_type());
@@ -265,8 +267,8 @@ py::tuple py_norm_residual(const Tensor& x, const Maybe& y, const Maybe& alpha, 
         value_check(kind >= 0, "gate must be ", shape_of({W}), ", ", shape_of(x.sizes()), " or ", shape_of(with_last(lead, 1)), ", got ", shape_of(gate->sizes()));
         type_check(gate->scalar_type() == (kind == CHANNEL ? at::kFloat : h_type), "a gate per channel is float32, any other of y's type: got ", gate->scalar_type());
     }
-    const Tensor xs = rows_of(x, W), ys = y ? rows_of(*y, y->size(-1)) : Tensor(), al = value(alpha), po = solid(value(post)), pr = solid(value(pre));
-    const Tensor gs = !gate ? Tensor() : kind == CHANNEL ? gate->contiguous() : rows_of(*gate, gate->size(-1));
+    const Tensor xs = rows_of(x, W), ys = y ? rows_of(*y, y->size(-1)) : Tensor(), al = plain(value(alpha)), po = solid(value(post)), pr = solid(value(pre));
+    const Tensor gs = !gate ? Tensor() : kind == CHANNEL ? solid(*gate) : rows_of(*gate, gate->size(-1));
     Tensor out, h;
     if (at::GradMode::is_enabled() && (wants(x) || wants(ys) || wants(al) || wants(po) || wants(gs) || wants(pr))) {
         auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
@@ -307,7 +309,7 @@ std::vector<Tensor> py_orthogonalize(const std::vector<Tensor>& mats, int64_t st
             if (outs[j].defined() || o.sizes() != m.sizes() || o.scalar_type() != m.scalar_type() || o.device() != m.device()) continue;
             outs[j] = at::empty(o.sizes(), o.options().requires_grad(false));
             if (!o.numel()) continue;
-            solids[j] = o.contiguous();
+            solids[j] = solid(o);
             in.push_back(solids[j].data_ptr()); out.push_back(outs[j].data_ptr());
         }
         if (in.empty()) continue;

@@ -135,3 +135,39 @@ def test_a_backward_pass_is_not_traced(name):
     with pytest.raises(NotImplementedError, match='traced'):
         make_fx(lambda g: torch.autograd.grad(out, x, g, retain_graph=True))(torch.ones_like(out))
     torch.autograd.grad(out, x, torch.ones_like(out))
+
+
+@pytest.mark.gpu
+def test_tensors_whose_sign_is_a_flag():
+    """The imaginary part of a conjugated tensor, dense or not, as any input and as a gradient: its values count, not what lies in memory."""
+    from boardlaw_amd import heads, networks, optim
+
+    def flagged(*shape):
+        z = torch.complex(torch.randn(shape, device='cuda'), torch.randn(shape, device='cuda'))
+        t = z.conj().imag
+        assert t.is_neg()
+        return t
+
+    dense = lambda t: torch._neg_view(t)
+    for W in (1, 12):
+        for lazy in (flagged(5, W), dense(torch.randn((5, W), device='cuda'))):
+            real = lazy.clone()
+            assert lazy.is_neg() and not real.is_neg()
+            same = lambda f: all(torch.equal(a, b) for a, b in zip(f(lazy), f(real)))
+            assert same(lambda t: heads.logprobs(t, torch.zeros(5, dtype=torch.int64, device='cuda'), k=2).values())
+            base, one = torch.randn((5, W), device='cuda'), torch.ones(W, device='cuda')
+            assert same(lambda t: networks.norm_residual(t, base, pre=one)) and same(lambda t: networks.norm_residual(base, t, pre=one))
+            assert same(lambda t: networks.norm_residual(base, base, gate=t)[:1]) and same(lambda t: networks.norm_residual(base, base, gate=t[:, :1])[:1])
+            assert same(lambda t: networks.norm_residual(base, base, None, t[0], t[1], t[2])) and same(lambda t: networks.norm_residual(base, base, t[0, 0])[:1])
+            assert same(lambda t: [optim.orthogonalize(t)])
+
+            def gradients(t):
+                x = base.detach().requires_grad_()
+                out, h = networks.norm_residual(x, base, pre=one)
+                o = heads.logprobs(x)
+                return torch.autograd.grad([out, h], x, [t, t], retain_graph=True) + torch.autograd.grad(o.entropy, x, t[:, 0])
+
+            assert same(gradients)
+    a = dense(torch.tensor([0, -3], device='cuda'))
+    x = torch.randn((2, 5), device='cuda')
+    assert torch.equal(heads.logprobs(x, a).logp, heads.logprobs(x, torch.tensor([0, 3], device='cuda')).logp)
