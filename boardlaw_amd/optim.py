@@ -73,7 +73,20 @@ class Muon(torch.optim.Optimizer):
 
 
 class Several(tuple):
-    """Optimisers that share a network's parameters out among them, as training.optimize takes them; saved and loaded as one (storage.save(opt=...))."""
+    """Optimisers that share a network's parameters out among them, as training.optimize takes them: saved and loaded as one (storage.save(opt=...)), and
+    one to a GradScaler, which looks through all parameter groups and steps all of them or none."""
+
+    @property
+    def param_groups(self):
+        return [group for o in self for group in o.param_groups]
+
+    def zero_grad(self, set_to_none=True):
+        for o in self:
+            o.zero_grad(set_to_none)
+
+    def step(self):
+        for o in self:
+            o.step()
 
     def state_dict(self):
         return {str(i): o.state_dict() for i, o in enumerate(self)}

@@ -11,7 +11,7 @@ import time
 import numpy as np
 import torch
 
-from . import arrdict, heads, learning, parallel
+from . import arrdict, heads, learning, optim, parallel
 
 
 def _sync(dev):
@@ -47,27 +47,27 @@ def losses(network, batch, entropy=0.):
 
 def optimize(network, scaler, opt, batch, sync_gradients=True, bucket=None, entropy=0.):
     """One learner step (main.py:76-98).  Returns (policy_loss, value_loss) as detached tensors.
-    opt: an optimiser, or several that share the network's parameters out among them.  entropy: see losses().
+    opt: an optimiser, or several that share the network's parameters out among them (a step is then skipped by all of them where any gradient
+    overflowed, as by one optimiser of all parameters).  entropy: see losses().
     bucket: a parallel.GradientBucket over `network` -- the gradients then live in one flat buffer that is zeroed, accumulated
     into, all-reduced and read by the optimiser in place (what `run` uses when there are several ranks)."""
     cuda = next(network.parameters()).is_cuda
-    opts = opt if isinstance(opt, (list, tuple)) else (opt,)
+    if isinstance(opt, (list, tuple)):
+        opt = optim.Several(opt)
     with torch.autocast('cuda', enabled=cuda):
         policy_loss, value_loss = losses(network, batch, entropy)
         loss = policy_loss + value_loss
     if bucket is not None:
         bucket.zero()
     else:
-        for o in opts:
-            o.zero_grad()
+        opt.zero_grad()
     scaler.scale(loss).backward()
     if sync_gradients:
         if bucket is not None:
             bucket.allreduce()
         else:
             parallel.allreduce_gradients(network)
-    for o in opts:
-        scaler.step(o)
+    scaler.step(opt)
     scaler.update()
     return policy_loss.detach(), value_loss.detach()
 
@@ -78,7 +78,6 @@ def make_optimizer(network, optimizer='adam', lr=1e-3, hidden_lr=0.02):
         return torch.optim.Adam(network.parameters(), lr=lr)
     if optimizer != 'muon':
         raise ValueError(f"optimizer must be 'adam' or 'muon', got {optimizer!r}")
-    from . import optim
     hidden, rest = optim.split(network)
     if not hidden:
         raise ValueError('the network has no residual blocks for Muon')

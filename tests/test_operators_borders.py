@@ -171,3 +171,35 @@ def test_tensors_whose_sign_is_a_flag():
     a = dense(torch.tensor([0, -3], device='cuda'))
     x = torch.randn((2, 5), device='cuda')
     assert torch.equal(heads.logprobs(x, a).logp, heads.logprobs(x, torch.tensor([0, 3], device='cuda')).logp)
+
+
+# ------------------------------------------------------------------------------------------------- a learner's step
+
+@pytest.mark.parametrize('where', ['policy.core.weight', 'body.1.weight'])
+@pytest.mark.parametrize('device,kind', [('cpu', 'list'), ('cpu', 'several'), pytest.param('cuda', 'muon', marks=pytest.mark.gpu)])
+def test_an_overflow_skips_every_optimiser(where, device, kind):
+    """An infinite gradient in one optimiser's parameters: no parameter moves and the scale goes down, as with one optimiser; then a step of all."""
+    from boardlaw_amd import arrdict, heads, networks, optim, training, validation
+    torch.manual_seed(0)
+    net = networks.FCModel(heads.Tensor((1,)), heads.Masked(2), width=8, depth=2).to(device)
+    with torch.no_grad():
+        for p in net.parameters():
+            if p.ndim == 0:
+                p.fill_(.4)
+    worlds = validation.All.initial(n_envs=16, n_seats=1, length=4, device=device)
+    logits = torch.log_softmax(torch.randn((16, 2), device=device), -1)
+    batch = arrdict.arrdict(worlds=worlds, decisions=arrdict.arrdict(logits=logits.half(), v=torch.randn((16, 1), device=device).half()), reward_to_go=torch.randn((16, 1), device=device).half())
+    hidden, rest = optim.split(net)
+    opt = training.make_optimizer(net, 'muon') if kind == 'muon' else [torch.optim.SGD(hidden, lr=.1), torch.optim.Adam(rest, lr=.1)]
+    opt = optim.Several(opt) if kind == 'several' else opt
+    scaler = torch.amp.GradScaler(device, init_scale=4., growth_interval=100)
+    before = {k: v.clone() for k, v in net.state_dict().items()}
+    hook = dict(net.named_parameters())[where].register_hook(lambda g: g * math.inf)
+    training.optimize(net, scaler, opt, batch)
+    assert all(torch.equal(v, before[k]) for k, v in net.state_dict().items()) and scaler.get_scale() == 2.
+    assert not any(o.state for o in opt)
+    hook.remove()
+    training.optimize(net, scaler, opt, batch)
+    after = net.state_dict()
+    assert not torch.equal(after['policy.core.weight'], before['policy.core.weight']) and not torch.equal(after['body.1.weight'], before['body.1.weight'])
+    assert all(torch.isfinite(v).all() for v in after.values()) and scaler.get_scale() == 2.
