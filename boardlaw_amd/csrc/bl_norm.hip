@@ -100,6 +100,50 @@ __device__ __forceinline__ Gate sigmoid(float g) {
     return {s, s == 0.f ? 0.f : e * s * s};
 }
 
+// Rows beyond 1.8e19, or under 1e-15 with an eps as small, have squares outside f32's range.  The kernel notes that one of its rows has, and
+// these come again behind its loop, from memory instead of registers, with the sums made of values scaled by a power of two.  (A branch behind each sum takes
+// registers with it: 8192 x 4096 bf16 34 -> 41 us)
+template <typename TX, typename TY, int G> __device__ __forceinline__ void odd_rows(const Norm& q, float* lds, int set) {
+    constexpr int ROWS = G > 256 ? 1 : 256 / G;
+    const int gl = threadIdx.x & (G - 1);
+    const float alpha = q.alpha ? *q.alpha : 1.f;
+    for (long r0 = (long)blockIdx.x * ROWS; r0 < q.R; r0 += (long)gridDim.x * ROWS) {
+        const long row = r0 + group_of<G>(), at = row < q.R ? row : q.R - 1;
+        const TX* x = (const TX*)q.x + at * q.xs;
+        const TY* y = (const TY*)q.y + at * q.ys;
+        bool odd = false;
+        auto inverse_rms = [&](auto value) {
+            auto mean = [&](float scale) {
+                float ss = 0.f;
+#pragma unroll 1
+                for (int j = gl; j < q.W; j += G) { const float v = value(j) * scale; ss = fmaf(v, v, ss); }
+                return row_sum<G>(ss, lds, set) * q.inv_w + q.eps * scale * scale;
+            };
+            const float first = mean(1.f), scale = first < 0x1p-100f ? 0x1p100f : first <= 0x1p126f ? 1.f : 0x1p-72f;
+            odd = odd || scale != 1.f;
+            return __builtin_amdgcn_rsqf(mean(scale)) * scale;
+        };
+        const float ry = q.post ? inverse_rms([&](int j) { return (float)y[j]; }) : 1.f;
+        auto x_out = [&](int j) {
+            if (!q.y) return (float)x[j];
+            float u = (float)y[j];
+            if (q.post) u *= q.post[j] * ry;
+            if (q.kind != BL_GATE_NONE)
+                u *= sigmoid(q.kind == BL_GATE_CHANNEL ? ((const float*)q.gate)[j] : (float)((const TY*)q.gate)[at * q.gs + (q.kind == BL_GATE_FULL ? j : 0)]).s;
+            return fmaf(alpha, u, (float)x[j]);
+        };
+        const float rx = q.pre ? inverse_rms(x_out) : 1.f;
+        if (!odd || row >= q.R) continue;
+#pragma unroll 1
+        for (int j = gl; j < q.W; j += G) {
+            const float v = x_out(j);
+            if (q.y) ((TX*)q.xo)[at * q.W + j] = (TX)v;
+            if (q.pre) ((TY*)q.h)[at * q.W + j] = (TY)(q.pre[j] * (v * rx));
+        }
+        if (q.stats && gl == 0) { q.stats[2 * at] = ry; q.stats[2 * at + 1] = rx; }
+    }
+}
+
 template <typename TX, typename TY, int G, int N, int VEC>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(Norm q) {
     __shared__ float lds[32];
@@ -111,6 +155,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(Norm q) {
     if (q.pre) read<G, VEC>(q.pre, gl, q.W, pre);
     if (q.kind == BL_GATE_CHANNEL) read<G, VEC>((const float*)q.gate, gl, q.W, gate);
     const float alpha = q.alpha ? *q.alpha : 1.f;
+    float least = 1.f, most = 1.f;              // reciprocals of rms
     for (long r0 = (long)blockIdx.x * ROWS; r0 < q.R; r0 += (long)gridDim.x * ROWS) {
         const long row = r0 + group_of<G>(), at = row < q.R ? row : q.R - 1;      // (G > 64: one row per workgroup, always live)
         const bool live = row < q.R;
@@ -158,7 +203,12 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(Norm q) {
             if (live) write<G, VEC>((TY*)q.h + at * q.W, gl, q.W, h);
         }
         if (q.stats && live && gl == 0) { q.stats[2 * at] = ry; q.stats[2 * at + 1] = rx; }
+        least = fminf(least, fminf(ry, rx)); most = fmaxf(most, fmaxf(ry, rx));
     }
+    const bool odd = least < 0x1p-63f || most > 0x1p50f;
+    if constexpr (G == 128) { if (!__syncthreads_or(odd)) return; }        // two rows, which share their barriers
+    else if (!__any(odd)) return;                                          // (a row of more lanes is its workgroup's only one: the same in every wave)
+    odd_rows<TX, TY, G>(q, lds, set);
 }
 
 // A lane's sums over its rows, for dpost, dpre and a gate per channel.  In registers; at 16 waves per workgroup, where a lane has 128 of them

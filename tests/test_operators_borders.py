@@ -203,3 +203,82 @@ def test_an_overflow_skips_every_optimiser(where, device, kind):
     after = net.state_dict()
     assert not torch.equal(after['policy.core.weight'], before['policy.core.weight']) and not torch.equal(after['body.1.weight'], before['body.1.weight'])
     assert all(torch.isfinite(v).all() for v in after.values()) and scaler.get_scale() == 2.
+
+
+# ------------------------------------------------------------------------------------------------------------ norm_residual
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('W', [2, 20, 100, 512, 600, 771, 1024, 1500, 4096, 8191, 8192])
+def test_norms_of_the_largest_and_smallest_rows(W, dtype):
+    """Rows whose sum of squares leaves f32's range, beside ordinary ones: h is pre times something of size 1 all the same, and every gradient the
+    formula's.  Seven rows: one of a shared wave or workgroup is extreme where the others are not."""
+    from boardlaw_amd import networks
+    torch.manual_seed(W)
+    base = torch.randn((7, W), device='cuda')
+    pre, post = 1 + .2 * torch.randn(W, device='cuda'), 1 + .2 * torch.randn(W, device='cuda')
+    gx = torch.randn((7, W), device='cuda')
+    # a row's sums: up to 24 + W / 512 roundings, as for ordinary rows; the scales are powers of two
+    k = 40 + W / 256
+    for powers, eps in (((0, 64, 100, 1, 70, 0, 122), 1e-5), ((0, -60, -100, 1, -80, 0, -118), 0.)):
+        scale = torch.tensor([2. ** p for p in powers], device='cuda', dtype=torch.float64)[:, None]
+        x = (base.double() * scale).to(dtype)
+        # the norm before a block
+        leaf = x.detach().requires_grad_()
+        _, h = networks.norm_residual(leaf, pre=pre, eps=eps)
+        g = gx.to(dtype)
+        d, = torch.autograd.grad(h, leaf, g)
+        want = x.double().requires_grad_()
+        rms = (want.square().mean(-1, keepdim=True) + eps).sqrt()
+        wh = pre.double() * want / rms
+        wd, = torch.autograd.grad(wh, want, g.double(), retain_graph=True)
+        assert (h.double() - wh).abs().le((half_step(dtype) + U * k) * wh.abs()).all()
+        # (the gradient's terms are of size |g pre| / rms, and cancel; beyond 2^100 it is a subnormal number or none: half of f32's smallest step)
+        size = (g.double() * pre).abs() / rms + (wh / pre).abs() * ((g.double() * wh).abs().mean(-1, keepdim=True) / rms)
+        assert (d.double() - wd).abs().le(half_step(dtype) * wd.abs() + U * 2 * k * size + 2. ** -133).all()
+        # the norm behind it: n is of size 1
+        leaf = x.detach().requires_grad_()
+        stream = torch.zeros((7, W), device='cuda', dtype=dtype)
+        out, _ = networks.norm_residual(stream, leaf, None, post, eps=eps)
+        d, = torch.autograd.grad(out, leaf, g)
+        wn = post.double() * want / rms
+        wd, = torch.autograd.grad(wn, want, g.double())
+        assert (out.double() - wn).abs().le((half_step(dtype) + U * k) * wn.abs()).all()
+        size = (g.double() * post).abs() / rms + (wn / post).abs() * ((g.double() * wn).abs().mean(-1, keepdim=True) / rms)
+        assert (d.double() - wd).abs().le(half_step(dtype) * wd.abs() + U * 2 * k * size + 2. ** -133).all()
+    # the extreme rows do not touch the others
+    x = base.clone()
+    plain = networks.norm_residual(x, pre=pre)[1]
+    x[3] *= 2. ** 100
+    other = networks.norm_residual(x, pre=pre)[1]
+    keep = [0, 1, 2, 4, 5, 6]
+    assert torch.equal(plain[keep], other[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('tx,ty', [(torch.float32, torch.float32), (torch.float32, torch.float16), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16)], ids=str)
+@pytest.mark.parametrize('W', [24, 90, 512, 700, 2000, 8192])
+def test_blocks_with_extreme_rows(W, tx, ty):
+    """The whole operator with every kind of gate on a stream, and a branch, of which some rows leave the range of squares."""
+    from boardlaw_amd import networks
+    from test_operators import norm_inputs, plain_norm
+    R = 9
+    k = 60 + W / 256
+    for kind in ('none', 'packed', 'full', 'channel', 'row'):
+        t, _ = norm_inputs(R, W, tx, ty, kind)
+        t['x'][4] = (t['x'][4].double() * 2. ** 90).to(tx)
+        if ty != torch.float16:
+            t['y'][7, :W] = (t['y'][7, :W].double() * 2. ** 90).to(ty)
+        with torch.no_grad():
+            for drop in ((), ('post',), ('pre',), ('alpha',)):
+                s = {n: None if n in drop else v for n, v in t.items()}
+                if 'post' in drop and ty != torch.float16:
+                    s['alpha'] = t['alpha'] * 2. ** -20                     # (the branch as it is)
+                out, h = networks.norm_residual(**s)
+                wo, wh = plain_norm(s['x'], s['y'], s['alpha'], s['post'], s['gate'], s['pre'], 1e-5)
+                size = wo.abs() + (wo - s['x'].double()).abs()
+                assert (out.double() - wo).abs().le(half_step(tx) * wo.abs() + U * k * size).all(), (kind, drop)
+                if wh is not None:
+                    # x_out's cancellation, through 1 / rms
+                    scale = wh.abs() + size * (s['pre'].double().abs() / (wo.square().mean(-1, keepdim=True) + 1e-5).sqrt())
+                    assert (h.double() - wh).abs().le(half_step(ty) * wh.abs() + 2 * U * k * scale + torch.finfo(ty).tiny * half_step(ty) * 2).all(), (kind, drop)
