@@ -119,10 +119,10 @@ struct LogProbsNode : torch::autograd::Function<LogProbsNode> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         once();
         const auto s = ctx->get_saved_variables();
-        const Tensor &raw = s[0], &actions = s[1], &valid = s[2], &top = s[3], &stats = s[4], &entropy = s[5];
-        const int64_t k = ctx->saved_data["k"].toInt();
+        const int64_t R = s[0].size(0), A = s[0].size(1), k = ctx->saved_data["k"].toInt();
+        // (a saved-tensor hook may return them with other strides)
+        const Tensor raw = rows_of(s[0], A), actions = solid(s[1]), valid = rows_of(s[2], A), top = solid(s[3]), stats = solid(s[4]), entropy = solid(s[5]);
         const bool given = ctx->saved_data["given"].toBool();
-        const int64_t R = raw.size(0), A = raw.size(1);
         const Tensor d = at::empty({R, A}, raw.options());
         if (R) {
             const Tensor g_entropy = solid(g[0]), g_logp = given ? solid(g[1]) : Tensor(), g_top = k ? solid(g[given ? 2 : 1]) : Tensor();
@@ -215,8 +215,10 @@ struct NormNode : torch::autograd::Function<NormNode> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         once();
         const auto s = ctx->get_saved_variables();
-        const Tensor &x = s[0], &y = s[1], &alpha = s[2], &post = s[3], &gate = s[4], &pre = s[5], &stats = s[6];
-        const int64_t kind = ctx->saved_data["kind"].toInt(), R = x.size(0), W = x.size(1);
+        const int64_t kind = ctx->saved_data["kind"].toInt(), R = s[0].size(0), W = s[0].size(1);
+        // (a saved-tensor hook may return them with other strides)
+        auto rows = [](const Tensor& t) { return t.defined() && t.dim() == 2 ? rows_of(t, t.size(1)) : solid(t); };
+        const Tensor x = rows(s[0]), y = rows(s[1]), alpha = plain(s[2]), post = solid(s[3]), gate = rows(s[4]), pre = solid(s[5]), stats = solid(s[6]);
         const at::ScalarType h_type = (at::ScalarType)ctx->saved_data["h_type"].toInt();
         const Tensor g_out = y.defined() ? rows_of(g[0], W) : Tensor(), g_h = pre.defined() ? rows_of(g.back(), W) : Tensor();
         auto like = [&](const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : Tensor(); };

@@ -282,3 +282,39 @@ def test_blocks_with_extreme_rows(W, tx, ty):
                     # x_out's cancellation, through 1 / rms
                     scale = wh.abs() + size * (s['pre'].double().abs() / (wo.square().mean(-1, keepdim=True) + 1e-5).sqrt())
                     assert (h.double() - wh).abs().le(half_step(ty) * wh.abs() + 2 * U * k * scale + torch.finfo(ty).tiny * half_step(ty) * 2).all(), (kind, drop)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('hook', ['on the cpu', 'transposed', 'checkpoint'])
+def test_saved_tensors_may_come_back_from_hooks(hook):
+    """What is saved for the backward pass goes through saved-tensor hooks, which may return it elsewhere in memory and with other strides: the same gradients.
+    (But for the order of sums: the columns from 5 on lie on 16-byte boundaries when they come back.  An entry's sums over 40 columns and 40 rows then differ
+    by 64 roundings each way of terms as large as the tensor's largest entry, a few of them joined, and can round to f16's next value.)"""
+    from torch.utils.checkpoint import checkpoint
+    from boardlaw_amd import heads, networks
+    torch.manual_seed(0)
+    wide, both = torch.randn((40, 3 * 48), device='cuda'), torch.randn((40, 2 * 40), device='cuda').half()
+    valid, actions = torch.rand((1, 48), device='cuda') < .8, torch.randint(0, 48, (40,), device='cuda')
+    alpha, post, pre, channel = torch.tensor(.7, device='cuda'), torch.rand(40, device='cuda'), torch.rand(40, device='cuda'), torch.randn(40, device='cuda')
+    element = torch.randn((40, 40), device='cuda').half()
+
+    def f(a, x, y, al, po, pr, ch, el):
+        o = heads.logprobs(a[:, 48:96], actions, valid, k=3)
+        return (o.logp, o.entropy, o.top_logp, *networks.norm_residual(x[:, 5:45], y, al, po, pre=pr), *networks.norm_residual(x[:, :40], y[:, :40], al, po, ch, pr),
+                *networks.norm_residual(x[:, :40], y[:, :40], al, po, el, pr))
+
+    def gradients(run, context):
+        leaves = [t.detach().clone().requires_grad_() for t in (wide, wide, both, alpha, post, pre, channel, element)]
+        torch.manual_seed(1)
+        with context:
+            outs = run(*leaves)
+        return torch.autograd.grad(outs, leaves, [torch.randn(o.shape, device='cuda').to(o.dtype) for o in outs])
+
+    import contextlib
+    turned = lambda t: t.t().contiguous().t() if t.dim() == 2 else torch.stack([t, t], -1)[..., 0]
+    context = {'on the cpu': lambda: torch.autograd.graph.save_on_cpu(), 'checkpoint': contextlib.nullcontext,
+               'transposed': lambda: torch.autograd.graph.saved_tensors_hooks(turned, lambda t: t)}[hook]()
+    run = f if hook != 'checkpoint' else lambda *leaves: checkpoint(f, *leaves, use_reentrant=False)
+    want = gradients(f, contextlib.nullcontext())
+    for a, b in zip(gradients(run, context), want):
+        assert (a.float() - b.float()).abs().le(4 * 64 * U * b.float().abs().amax() + 2 * half_step(b.dtype) * b.float().abs()).all()
