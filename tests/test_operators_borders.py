@@ -318,3 +318,81 @@ def test_saved_tensors_may_come_back_from_hooks(hook):
     want = gradients(f, contextlib.nullcontext())
     for a, b in zip(gradients(run, context), want):
         assert (a.float() - b.float()).abs().le(4 * 64 * U * b.float().abs().amax() + 2 * half_step(b.dtype) * b.float().abs()).all()
+
+
+def formula(t, g_out, g_h, eps=1e-5):
+    """networks.norm_residual and its gradients in 64 bits from their formulas, each with the sum of its terms' sizes (a term's own error is of its size: x_out's
+    cancellation counts with the sizes of what it is made of)."""
+    W = t['x'].shape[-1]
+    d = {n: None if v is None else v.detach().double() for n, v in t.items()}
+    x, alpha, post, pre = d['x'], d['alpha'], d['post'], d['pre']
+    y, gate = (d['y'][:, :W], d['y'][:, W:]) if d['y'].shape[-1] == 2 * W else (d['y'], d['gate'])
+    mean = lambda v: v.mean(-1, keepdim=True)
+    ry = 1 / (mean(y * y) + eps).sqrt()
+    n, s = y * ry, 1. if gate is None else torch.sigmoid(gate).expand_as(y)
+    u = s * post * n
+    out = x + alpha * u
+    rx = 1 / (mean(out * out) + eps).sqrt()
+    xn, xs = out * rx, (x.abs() + (alpha * u).abs()) * rx
+    gx, gh = g_out.double(), g_h.double()
+    tt = gh * pre
+    z, zs = gx + rx * (tt - xn * mean(tt * xn)), gx.abs() + rx * (tt.abs() + xs * mean((tt * xs).abs()))
+    dn, dns = alpha * z * s * post, (alpha * s * post).abs() * zs
+    dy, dys = ry * (dn - n * mean(dn * n)), ry * (dns + n.abs() * mean(dns * n.abs()))
+    want = dict(x=(z, zs), alpha=((z * u).sum(), (zs * u.abs()).sum()), post=((alpha * z * s * n).sum(0), ((alpha * s * n).abs() * zs).sum(0)), pre=((gh * xn).sum(0), (gh.abs() * xs).sum(0)))
+    if gate is not None:
+        dg, dgs = alpha * z * post * n * s * (1 - s), (alpha * post * n).abs() * zs * s * (1 - s)
+    if d['y'].shape[-1] == 2 * W:
+        dy, dys = torch.cat([dy, dg], -1), torch.cat([dys, dgs], -1)
+    elif gate is not None:
+        want['gate'] = (dg, dgs) if gate.shape == y.shape else (dg.sum(0), dgs.sum(0)) if gate.ndim == 1 else (dg.sum(-1, keepdim=True), dgs.sum(-1, keepdim=True))
+    want['y'] = dy, dys
+    return (out, x.abs() + (alpha * u).abs()), (pre * xn, pre.abs() * xs), want
+
+
+# more rows than one pass of all workgroups, forward (2048 workgroups) and backward (512), and a rest; 4, 16, 64, 128, 256, 512 and 1024 lanes a row
+MANY_ROWS = [(131200, 20), (131137, 24), (32900, 81), (33001, 88), (8300, 300), (8259, 512), (4201, 771), (4101, 776), (2100, 1501), (2099, 2048), (2061, 3001), (2070, 4096), (2055, 8191), (2051, 8192)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('R,W', MANY_ROWS)
+def test_norm_residual_of_many_rows(R, W):
+    """Every entry, and every column's sum over the rows, to within what its own terms allow: a row's sums have up to 24 + W / 512 roundings and every
+    term a few of them joined; a sum over rows one more for each of a lane's rows (under 8), a workgroup's 64 groups of lanes, 32 workgroups of a part, and 16 parts."""
+    from boardlaw_amd import networks
+    from test_operators import norm_inputs
+    k = 4 * (24 + W / 512)
+    for (tx, ty), kind in ((torch.float32, torch.float32), 'channel'), ((torch.float32, torch.float16), 'packed'), ((torch.bfloat16, torch.bfloat16), 'full'), ((torch.float32, torch.bfloat16), 'row'):
+        t, n = norm_inputs(R, W, tx, ty, kind)
+        t['y'][:, W // 3] *= 2. ** -12                                       # a small column beside the others
+        names = [a for a in t if t[a] is not None]
+        leaves = [t[a].requires_grad_() for a in names]
+        out, h = networks.norm_residual(**t)
+        g_out, g_h = (n(R, W) + .25 * t['y'][:, :W].detach().float()).to(tx), n(R, W).to(ty)
+        grads = dict(zip(names, torch.autograd.grad([out, h], leaves, [g_out, g_h])))
+        with torch.no_grad():
+            wo, wh, want = formula(t, g_out, g_h)
+            for name, got, (w, size), rows in [('out', out, wo, 0), ('h', h, wh, 0)] + [(a, grads[a], want[a], 0 if grads[a].shape[0:1] == (R,) else 120) for a in names]:
+                tol = half_step(got.dtype) * w.abs() + U * (k + rows) * size + torch.finfo(got.dtype).tiny * half_step(got.dtype) * 2
+                off = float(((got.double() - w).abs() / tol).max())
+                assert off <= 1, (kind, name, off)
+        del out, h, grads, want, wo, wh
+
+
+# ------------------------------------------------------------------------------------------------------- orthogonalize, larger
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('count,m,n', [(1, 33, 40), (2, 48, 64), (1, 64, 64), (2, 64, 128), (2, 100, 50), (1, 65, 65), (2, 65, 1000), (1, 100, 700), (3, 162, 512), (2, 512, 162), (1, 257, 257),
+                                       (35, 130, 140), (4, 512, 512), (9, 512, 512), (6, 1024, 512), (8, 1024, 1024)])
+def test_orthogonalize_is_as_exact_as_f32_products(count, m, n):
+    """Operands of 22 (33) bits and f32 sums: against 64 bits no more than 1.5 times as far off as the iteration in f32 products, on every spectrum; the low-rank
+    ones with noise are where operands of fewer bits fail (pairs of bf16 numbers: 40 times).  A matrix of its own spectrum each, more than one launch takes."""
+    from boardlaw_amd import optim
+    mats = [gradient_like(m, n, KINDS[i % 4], i).float() for i in range(max(count, 4))]
+    outs = optim.orthogonalize(mats[:count]) if count >= 4 else [optim.orthogonalize([g])[0] for g in mats]
+    for i, (g, o) in enumerate(zip(mats, outs)):
+        if i >= 12 and i % 8:
+            continue
+        want = iteration(g, torch.float64)
+        own, plain = float((o.double() - want).norm() / want.norm()), float((iteration(g, torch.float32).double() - want).norm() / want.norm())
+        assert own <= 1.5 * plain + U, (KINDS[i % 4], own / plain)
