@@ -396,3 +396,58 @@ def test_orthogonalize_is_as_exact_as_f32_products(count, m, n):
         want = iteration(g, torch.float64)
         own, plain = float((o.double() - want).norm() / want.norm()), float((iteration(g, torch.float32).double() - want).norm() / want.norm())
         assert own <= 1.5 * plain + U, (KINDS[i % 4], own / plain)
+
+
+# ------------------------------------------------------------------------------------------------- capture and build
+
+@pytest.mark.gpu
+def test_moves_are_captured_while_another_thread_asks_its_events():
+    """As an nccl process group's watchdog does: the captured moves are the eager ones, and the other thread sees no error."""
+    import threading
+    from boardlaw_amd import hex, networks
+    from boardlaw_amd.mcts import MCTSAgent
+    worlds = hex.Hex.initial(8, 4)
+    torch.manual_seed(0)
+    net = networks.FCModel(worlds.obs_space, worlds.action_space, width=16, depth=1).cuda()
+    event, done, errors, asked = torch.cuda.Event(), threading.Event(), [], []
+    event.record()
+    torch.cuda.synchronize()
+
+    def ask():
+        while not done.is_set():
+            try:
+                asked.append(event.query())
+            except Exception as e:
+                errors.append(e)
+                return
+
+    thread = threading.Thread(target=ask)
+    thread.start()
+    try:
+        agent = MCTSAgent(net, n_nodes=8, graph=True)
+        agent(worlds)
+        torch.manual_seed(3)
+        got = agent(worlds)
+        torch.cuda.synchronize()
+    finally:
+        done.set()
+        thread.join(30)
+    assert not errors and asked
+    eager = MCTSAgent(net, n_nodes=8)
+    eager(worlds)
+    torch.manual_seed(3)
+    want = eager(worlds)
+    assert torch.equal(got.actions, want.actions) and torch.equal(got.logits, want.logits)
+
+
+def test_no_packed_fp32_instructions(tmp_path):
+    """The build's flags keep the compiler from making them of ordinary float code, where it would."""
+    import subprocess
+    from boardlaw_amd import build
+    src = tmp_path / 'x.hip'
+    src.write_text('#include <hip/hip_runtime.h>\n__global__ void k(float2* x, float2 a) { float2 v = x[threadIdx.x]; v.x = v.x * a.x + a.y; v.y = v.y * a.x + a.y; '
+                   'x[threadIdx.x] = make_float2(v.x + a.x, v.y + a.x); }\n')
+    listing = lambda flags: subprocess.run([build._hipcc(), *flags, '-w', '--cuda-device-only', '-S', str(src), '-o', '-'], check=True, capture_output=True, text=True).stdout
+    flags = [f for f in build.FLAGS if f not in ('-Xclang', '-target-feature', '-packed-fp32-ops')]
+    packed = ('v_pk_add_f32', 'v_pk_mul_f32', 'v_pk_fma_f32')
+    assert any(p in listing(flags) for p in packed) and not any(p in listing(build.FLAGS) for p in packed)
