@@ -726,9 +726,13 @@ template <int MODE> bool multiply(const Product& p, const Mats& q, hipStream_t s
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     // The larger tile wherever it fills the chip well enough.  us for all 15 products of 5 steps on tiles of 64 x 64 / 128 x 128 / 256 x 128:
     // 8 matrices of 512: 220 / 256 / 389; of 1024, one: 206 / 338 / 557, two: 309 / 364 / 572, four: 502 / 443 / 596, eight: 845 / 840 / 757; one of 2048:
-    // 942 / 753 / 1010.  In tiles of these products: 256 x 128 pays from 160 of them on (72 .. 128 do not), 128 x 128 from 136 (72 .. 128 do not).
-    if (p.M % 256 == 0 && p.N % 128 == 0 && tiles_in<SYM, 256, 128>(p.M, p.N) * p.count >= 160) return wide<MODE, 4>(p, q, s);
-    if (p.M % 128 == 0 && p.N % 128 == 0 && tiles_in<SYM, 128, 128>(p.M, p.N) * p.count > 128) return wide<MODE, 2>(p, q, s);
+    // 942 / 753 / 1010.  128 x 128 pays from 136 tiles on (72 .. 128 do not), 256 x 128 where tiles of 128 x 128 are more than the 256 CUs and a second round
+    // of them begins.  Whole calls on 128 x 128 / 256 x 128, in tiles of 128 x 128 for X X^T: 24 x 512 x 1024, 240 tiles: 614 / 696; 7 x 1024 x 1024, 252: 587 / 693; 26 x 512 x 512, 260:
+    // 491 / 461; 2 x 2048 x 2048, 272: 1303 / 1219; B X alone, 3 x 1280 x 1280, 300: 597 / 542.
+    const bool whole = p.M % 128 == 0 && p.N % 128 == 0;
+    const int tiles = whole ? tiles_in<SYM, 128, 128>(p.M, p.N) * p.count : 0;
+    if (tiles > 256 && p.M % 256 == 0) return wide<MODE, 4>(p, q, s);
+    if (tiles > 128) return wide<MODE, 2>(p, q, s);
     hipLaunchKernelGGL((product_64_kernel<MODE>), dim3((unsigned)(tiles_in<SYM, 64, 64>(p.M, p.N) * p.count)), dim3(256), 65536, s, p, q);
     return true;
 }
