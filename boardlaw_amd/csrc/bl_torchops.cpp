@@ -83,6 +83,13 @@ void once() {
     TORCH_CHECK_NOT_IMPLEMENTED(!traced(), "this operator's backward pass cannot be traced");
 }
 
+// A saved tensor, or a gradient, as the kernels will read it: a saved-tensor hook may return anything
+void kept(const Tensor& t, const Tensor& first, at::IntArrayRef sizes, at::ScalarType type) {
+    TORCH_CHECK(!t.defined() || (t.is_cuda() && t.device() == first.device() && t.sizes() == sizes && t.scalar_type() == type),
+                "a saved tensor came back from its hook on another device or with another shape or type: ", t.device(), " ", t.scalar_type(), " ", shape_of(t.sizes()),
+                " instead of ", first.device(), " ", type, " ", shape_of(sizes));
+}
+
 // ---- log probabilities ----
 struct LogProbs { Tensor logp, entropy, top, top_logp, stats; };
 
@@ -108,7 +115,7 @@ struct LogProbsNode : torch::autograd::Function<LogProbsNode> {
         const LogProbs o = logprobs(raw, value(actions), value(valid), k, true);
         ctx->save_for_backward({raw, value(actions), value(valid), o.top, o.stats, o.entropy});
         ctx->set_materialize_grads(false);
-        ctx->saved_data["k"] = k;
+        ctx->saved_data["k"] = k; ctx->saved_data["A"] = raw.size(1);
         ctx->saved_data["given"] = o.logp.defined();
         if (o.top.defined()) ctx->mark_non_differentiable({o.top});
         variable_list out = {o.entropy};
@@ -119,13 +126,17 @@ struct LogProbsNode : torch::autograd::Function<LogProbsNode> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         once();
         const auto s = ctx->get_saved_variables();
-        const int64_t R = s[0].size(0), A = s[0].size(1), k = ctx->saved_data["k"].toInt();
+        TORCH_CHECK(s[0].dim() == 2 && code_of(s[0].scalar_type()) >= 0, "a saved tensor came back from its hook with another shape or type");
+        const int64_t R = s[0].size(0), A = ctx->saved_data["A"].toInt(), k = ctx->saved_data["k"].toInt();
+        kept(s[0], s[4], {R, A}, s[0].scalar_type());
+        kept(s[1], s[0], {R}, at::kLong); kept(s[2], s[0], {R, A}, at::kBool); kept(s[3], s[0], {R, k}, at::kLong); kept(s[4], s[0], {R, 2}, at::kFloat); kept(s[5], s[0], {R}, at::kFloat);
         // (a saved-tensor hook may return them with other strides)
         const Tensor raw = rows_of(s[0], A), actions = solid(s[1]), valid = rows_of(s[2], A), top = solid(s[3]), stats = solid(s[4]), entropy = solid(s[5]);
         const bool given = ctx->saved_data["given"].toBool();
         const Tensor d = at::empty({R, A}, raw.options());
         if (R) {
             const Tensor g_entropy = solid(g[0]), g_logp = given ? solid(g[1]) : Tensor(), g_top = k ? solid(g[given ? 2 : 1]) : Tensor();
+            kept(g_entropy, raw, {R}, at::kFloat); kept(g_logp, raw, {R}, at::kFloat); kept(g_top, raw, {R, k}, at::kFloat);
             const c10::DeviceGuard guard(raw.device());
             check(bl_logprobs_grad(ptr(raw), code_of(raw.scalar_type()), raw.stride(0), ptr<uint8_t>(valid), row_stride(valid), ptr<const long long>(actions), R, (int)A,
                                    (int)k, ptr<const long long>(top), ptr<float>(stats), ptr<float>(entropy), ptr<float>(g_logp), ptr<float>(g_entropy), ptr<float>(g_top),
@@ -215,12 +226,18 @@ struct NormNode : torch::autograd::Function<NormNode> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         once();
         const auto s = ctx->get_saved_variables();
+        TORCH_CHECK(s[0].dim() == 2 && code_of(s[0].scalar_type()) >= 0, "a saved tensor came back from its hook with another shape or type");
         const int64_t kind = ctx->saved_data["kind"].toInt(), R = s[0].size(0), W = s[0].size(1);
+        const at::ScalarType h_type = (at::ScalarType)ctx->saved_data["h_type"].toInt();
+        kept(s[0], s[6], {R, W}, s[0].scalar_type());
+        kept(s[1], s[0], {R, kind == PACKED ? 2 * W : W}, h_type); kept(s[2], s[0], {}, at::kFloat); kept(s[3], s[0], {W}, at::kFloat); kept(s[5], s[0], {W}, at::kFloat);
+        if (kind == CHANNEL) kept(s[4], s[0], {W}, at::kFloat); else kept(s[4], s[0], {R, kind == ROW ? 1 : W}, h_type);
+        kept(s[6], s[0], {R, 2}, at::kFloat);
         // (a saved-tensor hook may return them with other strides)
         auto rows = [](const Tensor& t) { return t.defined() && t.dim() == 2 ? rows_of(t, t.size(1)) : solid(t); };
         const Tensor x = rows(s[0]), y = rows(s[1]), alpha = plain(s[2]), post = solid(s[3]), gate = rows(s[4]), pre = solid(s[5]), stats = solid(s[6]);
-        const at::ScalarType h_type = (at::ScalarType)ctx->saved_data["h_type"].toInt();
         const Tensor g_out = y.defined() ? rows_of(g[0], W) : Tensor(), g_h = pre.defined() ? rows_of(g.back(), W) : Tensor();
+        kept(g_out, x, {R, W}, x.scalar_type()); kept(g_h, x, {R, W}, h_type);
         auto like = [&](const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : Tensor(); };
         const Tensor dx = like(x), dy = like(y);
         Tensor dalpha = like(alpha), dpost = like(post), dgate = like(gate), dpre = g_h.defined() ? like(pre) : Tensor();

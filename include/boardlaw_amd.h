@@ -440,7 +440,7 @@ int bl_logprobs_grad(const void* raw, int dtype, long raw_stride, const uint8_t*
  * x, x_out of x_dtype, y and h of y_dtype: equal, or x f32 and y f16 / bf16.  alpha: one f32 on the device, NULL = 1.  post, pre (W) f32.
  * gate by gate_kind: none (NULL); per element (R rows of W, y's type); per channel (W) f32; per row (one of y's type every gate_stride).
  * y NULL (then no gate, no post, x_out NULL): h = pre x / rms(x) only.  pre NULL: no h.  x_out, h contiguous.
- * stats_out (R,2) f32 or NULL: what the gradient call reads.  Computed in f32, each output rounded once. */
+ * stats_out (R,2) f32 or NULL: what the gradient call reads.  Outputs do not overlap inputs.  Computed in f32, each output rounded once. */
 #define BL_NORM_MAX 8192
 #define BL_GATE_NONE 0
 #define BL_GATE_FULL 1

@@ -451,3 +451,44 @@ def test_no_packed_fp32_instructions(tmp_path):
     flags = [f for f in build.FLAGS if f not in ('-Xclang', '-target-feature', '-packed-fp32-ops')]
     packed = ('v_pk_add_f32', 'v_pk_mul_f32', 'v_pk_fma_f32')
     assert any(p in listing(flags) for p in packed) and not any(p in listing(build.FLAGS) for p in packed)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('change', ['device', 'shape', 'type'])
+def test_saved_tensors_that_came_back_changed_are_refused(change):
+    """A hook that returns a saved tensor elsewhere, shorter or as another type: an error before anything is launched.  One tensor at a time."""
+    from boardlaw_amd import heads, networks
+    alter = dict(device=lambda t: t.cpu(), shape=lambda t: t[..., :-1] if t.dim() else t[None], type=lambda t: t.double() if t.is_floating_point() else t.int())[change]
+    x, y, w = torch.randn((6, 8), device='cuda'), torch.randn((6, 8), device='cuda').half(), torch.rand(8, device='cuda')
+    valid, actions = torch.ones((6, 8), dtype=torch.bool, device='cuda'), torch.zeros(6, dtype=torch.int64, device='cuda')
+    calls = [lambda: heads.logprobs(x.requires_grad_(), actions, valid, k=2).entropy]
+    calls += [lambda gate=gate: networks.norm_residual(x.requires_grad_(), y, torch.tensor(.5, device='cuda'), w, gate, w)[1] for gate in (y, w, y[:, :1], None)]
+    calls += [lambda: networks.norm_residual(x.requires_grad_(), torch.cat([y, y], -1), pre=w)[0], lambda: networks.norm_residual(x.requires_grad_(), pre=w)[1],
+              lambda: heads.logprobs(x.requires_grad_(), k=2).top_logp]
+    for call in calls:
+        count, at = 0, 0
+        while at <= count:                                                   # the at-th saved tensor; once more with none
+            seen = []
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: (len(seen), seen.append(0), t)[::2], lambda p: alter(p[1]) if p[0] == at else p[1]):
+                out = call()
+            count = len(seen)
+            if at < count:
+                with pytest.raises(RuntimeError, match='saved tensor|Expected all tensors'):
+                    torch.autograd.grad(out.sum(), x)
+            else:
+                torch.autograd.grad(out.sum(), x)
+            at += 1
+        assert count >= 3
+
+
+@pytest.mark.gpu
+def test_compiled_and_inference_mode_calls():
+    """torch.compile leaves the operators outside its graphs, and inference mode needs nothing of autograd: the eager results."""
+    f = calls('cuda')
+    for name, call in f.items():
+        x = torch.randn((3, 4), device='cuda')
+        want = call(x)
+        with torch.inference_mode():
+            assert torch.equal(call(x), want) and torch.equal(call(x.clone()), want)
+        torch._dynamo.reset()
+        assert torch.equal(torch.compile(lambda t: 2 * call(t + 0), backend='eager')(x), 2 * want)
