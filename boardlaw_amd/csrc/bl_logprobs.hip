@@ -7,9 +7,9 @@
 //     dx_j = g_a [j = a] + sum_i g_i [j = top_i] - p_j (g_a + sum_i g_i + g_H (logp_j + H)).
 // An invalid entry and a logit of -inf are the same thing: probability 0, never an alternative, gradient 0.
 //
-// One pass over the logits each way.  4096 x 32000 bf16: sums alone 67 us (262 MB at 3.9 TB/s, the VALU busy throughout: nine instructions and an exponential per
-// entry), with 4 alternatives 86 to 100, the gradient 91 us (524 MB, 5.8 TB/s).  32768 x 81 f16 with masks: 7.4 us and 6.3 us, 4.5 times the
-// bytes' time: instructions per row and the launch.
+// One pass over the logits each way.  4096 x 32000 bf16: sums alone 67 us (262 MB at 3.9 TB/s, the VALU busy throughout: 18 instructions per
+// entry by the counters, half of them the sums' own, most others the join of a new maximum), with 4 alternatives 100 us (23 per entry), the
+// gradient 94 us (524 MB, 5.6 TB/s).  32768 x 81 f16 with masks: 7.5 us and 6.5 us, 4.5 times the bytes' time: instructions per row and the launch.
 #include "bl_train.h"
 
 #pragma clang fp contract(off)

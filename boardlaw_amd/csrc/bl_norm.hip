@@ -9,7 +9,8 @@
 // is held in registers by G lanes of 8 elements each, so the two dependent sums of a row cost no second read.  The sums over rows are
 // kept per workgroup in registers over all of its rows and added up by a second launch in a fixed order: no atomics, the same bits
 // every time.  32768 x 512, f32 stream, f16 branches with gates: forward 42 us for 235 MB (5.5 TB/s), backward 68 us for 369 MB (5.4 TB/s) and
-// 4 us for the sums; 4096 x 771 f32 14 + 21 + 4 us; 8192 x 4096 bf16 forward 58 us for 335 MB (5.8 TB/s); a copy of 4 GiB runs at 4.75 TB/s, of 32 MiB at 6.6.
+// 4 us for the sums; 4096 x 771 f32 14 + 21 + 4 us; 8192 x 4096 bf16 forward 58 us for 335 MB (5.8 TB/s); a copy of 4 GiB runs at 4.75 TB/s, of 32 MiB at 6.6,
+// the data sheet says 8.
 #include "bl_train.h"
 #include "bl_host.h"
 

@@ -5,8 +5,8 @@
 // takes every singular value s to a s + b s^3 + c s^5 and again, i.e. towards 1.  The iteration multiplies what is small by up to 3.4 a
 // step: with f16 or bf16 operands the rounding of the large directions drowns the small ones of a low-rank gradient (3.7 % / 30 % of the
 // result on rank 8 + 1 % noise).  So every operand (beyond few rows, below) is a pair of f16 numbers hi + lo (22 bits and lo's sign), a product is hi hi + hi lo +
-// lo hi on v_mfma_f32_32x32x16_f16 with f32 sums (the dropped lo lo is 2^-24 of the product: what f32 rounding costs), 3/16 of the matrix
-// rate instead of the f32 MFMA's 1/16.  Operands carry a factor 2^13: entries of X and B stay below 3 (the quintic maps [0, 1.21] into
+// lo hi on v_mfma_f32_32x32x16_f16 with f32 sums (the dropped lo lo is up to 2^-22 of the product, 2^-24 typically: what f32 rounding costs), a third
+// of the f16 matrix rate where the f32 MFMA has a sixteenth.  Operands carry a factor 2^13: entries of X and B stay below 3 (the quintic maps [0, 1.21] into
 // itself), so hi < 2^15, and lo keeps its bits above f16's smallest steps down to entries of 2^-14.
 //
 // Operands lie in the workspace as MFMA fragments: 32 rows x 16 k, lane = row + 32 (k / 8), 8 consecutive k per lane, hi then lo -- a

@@ -29,7 +29,8 @@ def orthogonalize(matrices, steps=5, eps=1e-7):
 
 class Muon(torch.optim.Optimizer):
     """Momentum SGD whose update of every weight matrix is orthogonalised: m = momentum m + g, u = g + momentum m (nesterov) or m,
-    W = (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) orthogonalize(u).  For the two-dimensional weights of hidden layers."""
+    W = (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) orthogonalize(u).  For the two-dimensional weights of hidden layers.  m is held in the
+    weights' type, which is f32 in this package's networks."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0., steps=5):
         if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0:
