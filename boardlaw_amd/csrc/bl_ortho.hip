@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
     }
 }
 
-// ---- 32 < m <= 64 and n <= 64 NB <= 128: one workgroup takes a matrix through all of it in LDS ------------------------------------------------
+// ---- m <= 64 and n <= 64 NB <= 128 (mostly m > 32): one workgroup takes a matrix through all of it in LDS ------------------------------------------
 // 15 dependent products of a few hundred cycles each: launches (3 to 5 us apiece) would be nearly all of the time.  Here products cost next
 // to nothing, so operands are three f16 numbers (33 bits) and a product six: a small matrix is often nearly singular, and sums this
 // short leave f32 so little error of their own that 22 bits would show.
@@ -542,10 +542,12 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
 // Where it is used: up to 32 rows at any width, up to 64 beyond 128 wide.  us, beside the kernels above: 4 x 16 x 16 10.9 (19.2), 4 x 32 x 32 18.3 (21.2),
 // 4 x 8 x 400 15 (90), 4 x 32 x 200 27 (84), 4 x 64 x 300 85 (88), 64 x 1000 86 (102), 64 x 16384 133 (515); but 4 x 48 x 48 38 (23), 4 x 64 x 64 69 (25), 4 x 64 x 128 78 (41),
 // where three f16 numbers are as exact as f32.  The steps' f64 products bound it: 69 of 85 us at 64 x 300.
+// Up to 8 steps: a direction that G does not have is in A with its rounding, 2^-53 and of either sign, which a step multiplies by 3.4445^2; behind 8 of them it is
+// still nothing, behind 15 it would be as large as the others, and a negative one of that size diverges.  (X X^T has none: the kernels above take any number.)
 typedef double d4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ d4 mfma(double x, double y, d4 acc) { return __builtin_amdgcn_mfma_f64_16x16x4f64(x, y, acc, 0, 0, 0); }
 // rows of 16 MT doubles, an odd number of 16s apart: the four rows that a fragment's lanes read lie in different banks
-constexpr int ONE_PART = 256, MOST_PARTS = 32;
+constexpr int ONE_PART = 256, MOST_PARTS = 32, FEW_STEPS = 8;
 template <int MT> struct Few { static constexpr int MP = 16 * MT, LD = MP | 16, TILES = MT * (MT + 1) / 2, SIZE = MP * LD; };
 // tile t of those on and above the diagonal, column by column
 __device__ __forceinline__ void tile_at(int t, int& a, int& b) { b = 0; while (t > b) t -= ++b; a = t; }
@@ -710,7 +712,7 @@ Plan plan_of(int m, int n) {                // halves of one matrix: X (and each
     const long mp = up(m), np = up(n);
     return {2 * mp * np, 2 * mp * mp, MANY * PARTS * (long)sizeof(double)};
 }
-bool few_rows(int m, int n) { return m <= 32 || (m <= 64 && n > 128); }
+bool few_rows(int m, int n) { return m <= 32 || (m <= 64 && n > 128); }        // ... and up to FEW_STEPS
 // parts of a Gram matrix, by the columns alone (a matrix's result does not depend on its batch)
 int few_parts(int n) { return n <= ONE_PART ? 0 : (n + ONE_PART - 1) / ONE_PART < MOST_PARTS ? (n + ONE_PART - 1) / ONE_PART : MOST_PARTS; }
 long few_bytes(int count, int m, int n) { const long mp = (m + 15) / 16 * 16, s = few_parts(n); return count * (s > 0 ? s : 1) * mp * mp * (long)sizeof(double); }
@@ -757,7 +759,7 @@ template <typename T, int MT> int few(const Mats& q, int c, int m, int n, int ta
 template <typename T> int run(const Mats& q, int c, int m, int n, int tall, int dtype, int steps, float eps, const Plan& plan, void* workspace, hipStream_t s) {
     const int mp = up(m), np = up(n);
     double* parts = (double*)workspace;
-    if (few_rows(m, n))
+    if (few_rows(m, n) && steps <= FEW_STEPS)
         return m <= 16 ? few<T, 1>(q, c, m, n, tall, steps, eps, parts, s) : m <= 32 ? few<T, 2>(q, c, m, n, tall, steps, eps, parts, s)
              : m <= 48 ? few<T, 3>(q, c, m, n, tall, steps, eps, parts, s) : few<T, 4>(q, c, m, n, tall, steps, eps, parts, s);
     if (m <= 64 && n <= 128) {
@@ -793,7 +795,8 @@ long bl_orthogonalize_workspace(int count, int rows, int cols) {
     if (count <= 0 || rows <= 0 || cols <= 0 || rows > BL_ORTHO_MAX || cols > BL_ORTHO_MAX) return 0;
     const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
     if (count > MANY) count = MANY;
-    return few_rows(m, n) ? few_bytes(count, m, n) : plan_of(m, n).total(count);
+    const long all = plan_of(m, n).total(count), few = few_rows(m, n) ? few_bytes(count, m, n) : 0;       // (whatever the steps)
+    return all > few ? all : few;
 }
 
 int bl_orthogonalize(const void* const* host_in, void* const* host_out, int count, int dtype, int rows, int cols, int steps, float eps,

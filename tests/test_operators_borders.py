@@ -492,3 +492,57 @@ def test_compiled_and_inference_mode_calls():
             assert torch.equal(call(x), want) and torch.equal(call(x.clone()), want)
         torch._dynamo.reset()
         assert torch.equal(torch.compile(lambda t: 2 * call(t + 0), backend='eager')(x), 2 * want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('m,n', [(16, 16), (20, 700), (64, 300), (50, 60)])
+def test_few_rows_on_streams_and_in_graphs(m, n):
+    """Two captured graphs, replayed in turn on new matrices between eager calls on two streams: every result the eager one's."""
+    from boardlaw_amd import optim
+    mats = lambda seed: [gradient_like(m, n, KINDS[i % 4], 10 * seed + i).float() for i in range(5)]
+    want = {s: optim.orthogonalize(mats(s)) for s in range(4)}
+    graphs = []
+    for _ in range(2):
+        static = mats(0)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            optim.orthogonalize(static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = optim.orthogonalize(static)
+        graphs.append((graph, static, outs))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in (1, 2, 3, 1):
+        inputs = mats(s)
+        torch.cuda.synchronize()
+        got = []
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got.append(optim.orthogonalize(inputs))
+        for graph, static, outs in graphs:
+            for dst, src in zip(static, inputs):
+                dst.copy_(src)
+            graph.replay()
+        torch.cuda.synchronize()
+        for result in got + [outs for _, _, outs in graphs]:
+            assert all(torch.equal(a, b) for a, b in zip(result, want[s]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('m,n', [(8, 8), (20, 24), (20, 700), (300, 17), (64, 300), (50, 60)])
+def test_orthogonalize_with_other_numbers_of_steps(m, n):
+    """One step to many, also of matrices of lower rank, whose missing directions must not grow out of roundings: no singular value passes the quintic's
+    largest, 1.2023.  Up to 8 steps also the value itself (later a rounding is multiplied by more than 1.5 in each step: the quintic at its fixed point)."""
+    from boardlaw_amd import optim
+    one, two = torch.ones((m, n), device='cuda'), gradient_like(m, 2, 'randn', 1).float() @ gradient_like(2, n, 'randn', 2).float()
+    for g in (gradient_like(m, n, 'randn', 3).float(), gradient_like(m, n, 'decay', 4).float(), one, two):
+        for steps in (1, 2, 3, 8, 9, 12, 16, 20, 40):
+            out = optim.orthogonalize(g, steps=steps).double()
+            assert torch.isfinite(out).all() and torch.linalg.matrix_norm(out, 2) <= 1.2023 * (1 + 1e-4), steps
+            if steps <= 8:
+                # A step adds a X, b A X and c A^2 X, where |X| and |A| go up to 1: a rounding of A counts 4.7750 times and twice 2.0315, one of A^2 2.0315,
+                # of B X 4.7750 - 2.0315, of a X 3.4445: 17 in all, each of f32's size, or of 22 bits; times at most 3.4445 in each step behind it
+                want = iteration(g, torch.float64, steps)
+                assert (out - want).norm() <= 17 * U * steps * 3.4445 ** (steps - 1) * max(1., float(want.norm()))
