@@ -542,12 +542,13 @@ __global__ void __launch_bounds__(256) ortho_small_kernel(Mats q, Product p, int
 // Where it is used: up to 32 rows at any width, up to 64 beyond 128 wide.  us, beside the kernels above: 4 x 16 x 16 10.9 (19.2), 4 x 32 x 32 18.3 (21.2),
 // 4 x 8 x 400 15 (90), 4 x 32 x 200 27 (84), 4 x 64 x 300 85 (88), 64 x 1000 86 (102), 64 x 16384 133 (515); but 4 x 48 x 48 38 (23), 4 x 64 x 64 69 (25), 4 x 64 x 128 78 (41),
 // where three f16 numbers are as exact as f32.  The steps' f64 products bound it: 69 of 85 us at 64 x 300.
-// Up to 8 steps: a direction that G does not have is in A with its rounding, 2^-53 and of either sign, which a step multiplies by 3.4445^2; behind 8 of them it is
-// still nothing, behind 15 it would be as large as the others, and a negative one of that size diverges.  (X X^T has none: the kernels above take any number.)
+// Up to 6 steps: a direction that G does not have is in A with its rounding, 2^-53 and of either sign, which a step multiplies by 3.4445^2, and in Q with 3.4445 a step:
+// 41 times a step in Q G.  Ones of 20 x 24 are 7e-9, 4e-8, 2e-6, 6e-5 off behind 5, 6, 7, 8 steps (the f32 form 3e-6) and diverge behind 12; X X^T has no such
+// direction, and the kernels above take any number of steps.
 typedef double d4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ d4 mfma(double x, double y, d4 acc) { return __builtin_amdgcn_mfma_f64_16x16x4f64(x, y, acc, 0, 0, 0); }
 // rows of 16 MT doubles, an odd number of 16s apart: the four rows that a fragment's lanes read lie in different banks
-constexpr int ONE_PART = 256, MOST_PARTS = 32, FEW_STEPS = 8;
+constexpr int ONE_PART = 256, MOST_PARTS = 32, FEW_STEPS = 6;
 template <int MT> struct Few { static constexpr int MP = 16 * MT, LD = MP | 16, TILES = MT * (MT + 1) / 2, SIZE = MP * LD; };
 // tile t of those on and above the diagonal, column by column
 __device__ __forceinline__ void tile_at(int t, int& a, int& b) { b = 0; while (t > b) t -= ++b; a = t; }

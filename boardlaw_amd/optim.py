@@ -13,7 +13,7 @@ def orthogonalize(matrices, steps=5, eps=1e-7):
         matrices  a tensor (..., m, n), or a list of matrices (m, n) of any shapes: f32, f16 or bf16, sides up to 16384
 
     -> the same structure, types and shapes; as exact as f32 products whatever the type (22-bit operands and f32 sums; f64 for a shorter side of up to
-    32, or up to 64 beside more than 128, and up to 8 steps).  Matrices of one shape and type are taken through it together.  Not differentiable.  On the GPU only (bl_orthogonalize)."""
+    32, or up to 64 beside more than 128, and up to 6 steps).  Matrices of one shape and type are taken through it together.  Not differentiable.  On the GPU only (bl_orthogonalize)."""
     if not isinstance(matrices, torch.Tensor):
         return _native.ops().orthogonalize(matrices, steps, eps)
     if matrices.ndim < 2:

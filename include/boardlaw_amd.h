@@ -465,7 +465,7 @@ int bl_norm_residual_grad(const void* x, int x_dtype, long x_stride, const void*
  * X = a X + (b A + c A^2) X with A = X X^T, (a, b, c) = (3.4445, -4.7750, 2.0315) -- singular values go to about 1 (0.7 .. 1.2 after five
  * steps).  host_in / host_out: HOST arrays of device pointers to contiguous row-major matrices of dtype, read before the call returns; in and out may be the
  * same.  Whatever dtype, operands are held to 22 bits and summed in f32 (33 bits up to 64 x 128; f64 throughout for a
- * shorter side of up to 32, or up to 64 beside more than 128, and up to 8 steps); the result is rounded once.  A zero matrix gives zeros.
+ * shorter side of up to 32, or up to 64 beside more than 128, and up to 6 steps); the result is rounded once.  A zero matrix gives zeros.
  * workspace: bl_orthogonalize_workspace(count, rows, cols) bytes, 16-byte aligned, this call's own until its work on `stream` is done. */
 #define BL_ORTHO_MAX 16384
 long bl_orthogonalize_workspace(int count, int rows, int cols);

@@ -546,3 +546,19 @@ def test_orthogonalize_with_other_numbers_of_steps(m, n):
                 # of B X 4.7750 - 2.0315, of a X 3.4445: 17 in all, each of f32's size, or of 22 bits; times at most 3.4445 in each step behind it
                 want = iteration(g, torch.float64, steps)
                 assert (out - want).norm() <= 17 * U * steps * 3.4445 ** (steps - 1) * max(1., float(want.norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('m,n', [(8, 8), (20, 24), (20, 700), (17, 300), (32, 16384), (64, 300), (4000, 8)])
+def test_few_rows_of_lower_rank(m, n):
+    """f64 on the m x m side, up to 6 steps: a rounding in A (products of up to 64 terms, two in a row: 16 at random) comes out 3.4445^3 = 41 times as
+    large for each step behind it where the matrix lacks a direction, which is still f32's size."""
+    from boardlaw_amd import optim
+    row = gradient_like(1, n, 'randn', 5)
+    mats = dict(ones=torch.ones((m, n), device='cuda'), same=row.expand(m, n), rank2=gradient_like(m, 2, 'randn', 1) @ gradient_like(2, n, 'randn', 2),
+                one_row=torch.cat([row, torch.zeros((m - 1, n), device='cuda')]), steep=gradient_like(m, n, 'steep', 3))
+    for name, g in mats.items():
+        for steps in (1, 2, 3, 4, 5, 6):
+            out, want = optim.orthogonalize(g.float(), steps=steps).double(), iteration(g.float(), torch.float64, steps)
+            off = float((out - want).norm() / want.norm())
+            assert off <= U + 16 * 2. ** -53 * 41. ** (steps - 1), (name, steps, off)
